@@ -11,8 +11,8 @@
  *     calling thread's last error; per device, created on first use and guarded by mutexes so that several
  *     host threads may drive several GPUs: one side stream with two events (kvm_decode_step's overlapped
  *     memory update), a small cache of tensor maps keyed by the decode cache's addresses and sizes, the
- *     shared-memory limits already raised on the kernels, cached occupancy answers, and the device address
- *     of the built-in scratch of kvm_decode_step_static.  None of it depends on the data of a call;
+ *     shared-memory limits already raised on the kernels, cached occupancy answers, and the device addresses
+ *     of the built-in scratch of kvm_decode_step_static and of the window operators' status word.  None of it depends on the data of a call;
  *   - all activations and memory rows are bfloat16, lengths/norms fp32, indices int32;
  *   - `stream` is a cudaStream_t passed as void* (NULL = default stream); calls only enqueue work;
  *   - return value 0 = ok, otherwise one of KVM_ERR_*; kvm_last_error_string() describes the last
@@ -424,6 +424,63 @@ int kvm_memory_refresh(const kvm_layer* layer, int32_t batch, kvm_memory memory,
  * [B, T, H*D] with the heads in rank order.  shard_bytes a multiple of 16, both buffers 16-byte aligned.
  * No counterpart in the reference (its mixers run on one device); replaces a strided tensor copy in the host code. */
 int kvm_interleave_shards(void* dst, const void* src, int32_t n_shards, int64_t n_tokens, int64_t shard_bytes, void* stream);
+
+/* ---- Sliding-window operators --------------------------------------------------------------------------------------
+ * Attention in which a token at position p sees position j if j <= p and (j > p - window or j < sinks): the last `window`
+ * tokens, itself among them, and the first `sinks` tokens of its sequence.  Prompts (kvm_window_attention) and single tokens
+ * over a cache of those tokens (kvm_window_attend), held in 16 or in 4 bits.  No counterpart at this boundary in the
+ * reference: its sliding-window mixers (model/swa_mixer.py) call library attention over uncompressed caches.
+ *
+ * Rows of a kv row's cache: the first tokens in row = position, `sinks` rounded up to 16 of them; behind them a ring of
+ * `window` rows rounded up to 16.
+ *   bits 16: k and v are bf16 [batch * n_kv_heads][rows][head_dim].
+ *   bits 4:  k holds keys and values in blocks of 16 rows (18 * head_dim bytes each), v is not used.  Groups of 32 channels
+ *            share a scale, a sixth of the largest magnitude rounded to 6 significant bits; a value is the nearest of
+ *            0, .5, 1, 1.5, 2, 3, 4, 6 (either sign) to value / scale, ties to even.  What stands there is a bf16 number and
+ *            comes back unchanged.  A group with an infinity or NaN reads back as NaN; one whose scale would be below 2^-126
+ *            as zeros.
+ * The arrays start as zeros (the caller clears them once). */
+typedef struct kvm_window_cache {
+  int32_t batch, n_kv_heads, head_dim;   /* head_dim 32, 64 or 128 */
+  int32_t window, sinks, bits;
+  void* k;                               /* kvm_window_cache_bytes() each */
+  void* v;
+} kvm_window_cache;
+
+/* Bytes of each of the cache's arrays (0: bad description). */
+size_t kvm_window_cache_bytes(const kvm_window_cache* cache);
+
+/* Writes tokens [position, position + length) of every sequence: k, v [batch, n_kv_heads, n_tokens, head_dim], of which the
+ * first `length` are taken.  positions_dev / lengths_dev: int32 [batch] on the device, or NULL: `position` / `length` for all
+ * sequences.  A negative position, or a length of 0, leaves the sequence as it is.  Tokens that later tokens of the same
+ * call push out are not written.  Positions stay below 2^31 - n_tokens. */
+int kvm_window_cache_write(const kvm_window_cache* cache, kvm_tensor4 k, kvm_tensor4 v, int64_t n_tokens, const int32_t* positions_dev,
+                           int32_t position, const int32_t* lengths_dev, int32_t length, void* stream);
+
+/* What the cache holds of sequences of `length` tokens, in order: k_out, v_out bf16 [batch, n_kv_heads, sinks + window, head_dim],
+ * the first sinks tokens, then the last `window`, zeros behind them. */
+int kvm_window_cache_read(const kvm_window_cache* cache, const int32_t* lengths_dev, int32_t length, void* k_out, void* v_out, void* stream);
+
+/* One query per sequence: q [batch, n_q_heads, 1, head_dim], out bf16 [batch, n_q_heads * head_dim]; at most 16 query heads per
+ * kv head.  Without a new token (k_new.ptr and v_new.ptr NULL) lengths are the tokens of the sequences, the query's own among
+ * them; with one they are its positions, and it is written to the cache on the way.  A sequence of no tokens (length 0, or
+ * position -1) gets zeros.  The workspace holds partial results of one call; calls in flight at the same time need one each. */
+size_t kvm_window_attend_workspace_bytes(const kvm_window_cache* cache, int32_t n_q_heads);
+int kvm_window_attend(const kvm_window_cache* cache, int32_t n_q_heads, kvm_tensor4 q, kvm_tensor4 k_new, kvm_tensor4 v_new,
+                      const int32_t* lengths_dev, int32_t length, float scale, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* A prompt, or a chunk of one behind earlier tokens: q [batch, n_q_heads, n_queries, head_dim], k, v [batch, n_kv_heads, n_keys,
+ * head_dim], out bf16 [batch, n_queries, n_q_heads * head_dim].  Query t stands at position n_keys - n_queries + t.
+ * lengths_dev (int32 [batch], or NULL: n_keys): tokens of each sequence; tokens behind them are padding, never looked at, and
+ * their output rows are zeros. */
+int kvm_window_attention(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_queries, int64_t n_keys,
+                         kvm_tensor4 q, kvm_tensor4 k, kvm_tensor4 v, int64_t window, int64_t sinks, float scale,
+                         const int32_t* lengths_dev, void* out, void* stream);
+
+/* Device-side condition of the window kernels on the current device since the last call (synchronises the stream):
+ * KVM_ERR_DEVICE_TIMEOUT if a bounded wait ran out.  One word per device, in the library. */
+int kvm_window_status(void* stream);
 
 /* Description of the last error of the calling thread ("" if none). */
 const char* kvm_last_error_string(void);

@@ -92,6 +92,11 @@ class KvmPromptCall(C.Structure):
                 ("workspace_bytes", C.c_size_t)]
 
 
+class KvmWindowCache(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("window", C.c_int32), ("sinks", C.c_int32), ("bits", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
 EXPORTS = [
     "kvm_prefill_workspace_bytes", "kvm_prefill_forward", "kvm_decode_workspace_bytes", "kvm_decode_step",
     "kvm_memory_refresh", "kvm_last_error_string", "kvm_abi_version", "kvm_decode_step_static", "kvm_prefill_status", "kvm_decode_run",
@@ -99,6 +104,8 @@ EXPORTS = [
     "kvm_prefill_forward_gathered", "kvm_decode_step_call", "kvm_decode_span",
     "kvm_decode_cache_fill", "kvm_project", "kvm_token_scratch_bytes", "kvm_mixer_token",
     "kvm_prompt_workspace_bytes", "kvm_mixer_prompt",
+    "kvm_window_cache_bytes", "kvm_window_cache_write", "kvm_window_cache_read", "kvm_window_attend_workspace_bytes",
+    "kvm_window_attend", "kvm_window_attention", "kvm_window_status",
 ]
 STATIC_SCRATCH_BYTES = 32 << 20
 PROJECT_ROWS_MAX = 128  # rows of one kvm_project
@@ -179,6 +186,23 @@ def load():
                                 C.c_int64, C.c_void_p]
     lib.kvm_interleave_shards.restype = C.c_int
     lib.kvm_interleave_shards.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p]
+    lib.kvm_window_cache_bytes.restype = C.c_size_t
+    lib.kvm_window_cache_bytes.argtypes = [LP(KvmWindowCache)]
+    lib.kvm_window_cache_write.restype = C.c_int
+    lib.kvm_window_cache_write.argtypes = [LP(KvmWindowCache), KvmTensor4, KvmTensor4, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p,
+                                           C.c_int32, C.c_void_p]
+    lib.kvm_window_cache_read.restype = C.c_int
+    lib.kvm_window_cache_read.argtypes = [LP(KvmWindowCache), C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.kvm_window_attend_workspace_bytes.restype = C.c_size_t
+    lib.kvm_window_attend_workspace_bytes.argtypes = [LP(KvmWindowCache), C.c_int32]
+    lib.kvm_window_attend.restype = C.c_int
+    lib.kvm_window_attend.argtypes = [LP(KvmWindowCache), C.c_int32, KvmTensor4, KvmTensor4, KvmTensor4, C.c_void_p, C.c_int32, C.c_float,
+                                      C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.kvm_window_attention.restype = C.c_int
+    lib.kvm_window_attention.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, KvmTensor4, KvmTensor4,
+                                         KvmTensor4, C.c_int64, C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.kvm_window_status.restype = C.c_int
+    lib.kvm_window_status.argtypes = [C.c_void_p]
     lib.kvm_last_error_string.restype = C.c_char_p
     lib.kvm_last_error_string.argtypes = []
     lib.kvm_abi_version.restype = C.c_int

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "kvm_common.cuh"
+#include "kvm_window.cuh"
 
 namespace kvm {
 cudaError_t prefill_dispatch(int D, const LayerDev& L, int batch, long long T, Tensor4 q, Tensor4 k, Tensor4 v,
@@ -27,6 +28,14 @@ cudaError_t cache_fill_dispatch(int D, const LayerDev& L, int batch, long long T
                                 int rows, const DecodeCacheDev& cache, int* counters, int n_counters, cudaStream_t stream);
 cudaError_t refresh_dispatch(int D, const LayerDev& L, int batch, MemoryDev mem, const int* state_len,
                              cudaStream_t stream);
+cudaError_t window_write_dispatch(int D, int bits, const WindowDev& W, Tensor4 k, Tensor4 v, int n_tokens, SeqInts positions,
+                                  SeqInts lengths, cudaStream_t stream);
+cudaError_t window_read_dispatch(int D, int bits, const WindowDev& W, SeqInts lengths, bf16* k_out, bf16* v_out, cudaStream_t stream);
+size_t window_token_workspace(int D, int G);
+cudaError_t window_token_dispatch(int D, int bits, const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens,
+                                  float scale, float* partial, bf16* out, int* status, cudaStream_t stream);
+cudaError_t window_prompt_dispatch(int D, int batch, int Hq, int Hkv, int T, int S, Tensor4 q, Tensor4 k, Tensor4 v, int window,
+                                   int sinks, float scale, const int* lengths, bf16* out, int* status, cudaStream_t stream);
 }  // namespace kvm
 
 using namespace kvm;
@@ -196,6 +205,68 @@ int static_scratch_for_current_device(void** out) {
     g_static_ptr[dev] = p;
   }
   *out = g_static_ptr[dev];
+  return KVM_OK;
+}
+
+// ---- sliding-window operators
+__device__ int g_window_status;  // set by a window kernel whose bounded wait ran out
+int* g_window_status_ptr[kMaxDevices] = {nullptr};
+
+int window_status_word(int** out) {
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "window operators: cudaGetDevice");
+  if (dev < 0 || dev >= kMaxDevices) return fail(KVM_ERR_UNSUPPORTED, "window operators: device ordinal %d not supported", dev);
+  std::lock_guard<std::mutex> lock(g_static_mu);
+  if (!g_window_status_ptr[dev]) {
+    void* p = nullptr;
+    e = cudaGetSymbolAddress(&p, g_window_status);
+    if (e != cudaSuccess) return cuda_fail(e, "window operators: cudaGetSymbolAddress");
+    g_window_status_ptr[dev] = static_cast<int*>(p);
+  }
+  *out = g_window_status_ptr[dev];
+  return KVM_OK;
+}
+
+WindowDev window_dev(const kvm_window_cache* c) {
+  WindowDev w;
+  w.batch = c->batch; w.Hkv = c->n_kv_heads; w.window = c->window; w.sinks = c->sinks;
+  w.sp = (c->sinks + 15) / 16 * 16;
+  w.ring = (c->window + 15) / 16 * 16;
+  w.rows = w.sp + w.ring;
+  w.k = w.v = nullptr;
+  w.blocks = nullptr;
+  if (c->bits == 4) {
+    w.blocks = static_cast<unsigned char*>(c->k);
+  } else {
+    w.k = static_cast<bf16*>(c->k);
+    w.v = static_cast<bf16*>(c->v);
+  }
+  return w;
+}
+
+int check_window(const kvm_window_cache* c, bool arrays) {
+  if (!c) return fail(KVM_ERR_BAD_ARGUMENT, "cache is NULL");
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128)
+    return fail(KVM_ERR_UNSUPPORTED, "head_dim %d not supported (32, 64 or 128)", c->head_dim);
+  if (c->bits != 4 && c->bits != 16) return fail(KVM_ERR_UNSUPPORTED, "a window cache holds 4 or 16 bits per value, not %d", c->bits);
+  if (c->batch <= 0 || c->n_kv_heads <= 0) return fail(KVM_ERR_BAD_ARGUMENT, "batch %d and n_kv_heads %d must be positive", c->batch, c->n_kv_heads);
+  if (c->window < 1 || c->sinks < 0 || c->window > (1 << 30) || c->sinks > (1 << 29))
+    return fail(KVM_ERR_BAD_ARGUMENT, "window %d must be in [1, 2^30], sinks %d in [0, 2^29]", c->window, c->sinks);
+  const WindowDev w = window_dev(c);
+  if ((int64_t)c->batch * c->n_kv_heads > (1 << 24) || (int64_t)c->batch * c->n_kv_heads * w.rows > 0x7fffffff)
+    return fail(KVM_ERR_CAPACITY, "%d x %d kv rows of %d cache rows each: 2^24 kv rows and 2^31 - 1 cache rows at most", c->batch, c->n_kv_heads,
+                w.rows);
+  if (arrays && (!c->k || ((uintptr_t)c->k) % 16 || (c->bits == 16 && (!c->v || ((uintptr_t)c->v) % 16))))
+    return fail(KVM_ERR_BAD_ARGUMENT, "the cache's arrays must be 16-byte aligned and not NULL");
+  return KVM_OK;
+}
+
+int check_groups(const kvm_window_cache* c, int n_q_heads) {
+  if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads)
+    return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, c->n_kv_heads);
+  if (n_q_heads / c->n_kv_heads > 16)
+    return fail(KVM_ERR_UNSUPPORTED, "%d query heads per kv head (at most 16)", n_q_heads / c->n_kv_heads);
   return KVM_OK;
 }
 
@@ -447,6 +518,114 @@ int kvm_project(const void* x, int64_t x_stride, int32_t n_rows, int32_t width, 
                 int32_t n_weights, void* out, int64_t out_stride, void* stream) {
   g_err[0] = 0;
   return project_impl(x, x_stride, n_rows, width, weights, weight_rows, n_weights, out, out_stride, stream, false);
+}
+
+size_t kvm_window_cache_bytes(const kvm_window_cache* cache) {
+  g_err[0] = 0;
+  if (check_window(cache, false)) return 0;
+  const size_t rows = (size_t)cache->batch * cache->n_kv_heads * window_dev(cache).rows;
+  return cache->bits == 4 ? rows / 16 * 18 * cache->head_dim : rows * cache->head_dim * 2;
+}
+
+size_t kvm_window_attend_workspace_bytes(const kvm_window_cache* cache, int32_t n_q_heads) {
+  g_err[0] = 0;
+  if (check_window(cache, false) || check_groups(cache, n_q_heads)) return 0;
+  return window_token_workspace(cache->head_dim, n_q_heads / cache->n_kv_heads);
+}
+
+int kvm_window_cache_write(const kvm_window_cache* cache, kvm_tensor4 k, kvm_tensor4 v, int64_t n_tokens, const int32_t* positions_dev,
+                           int32_t position, const int32_t* lengths_dev, int32_t length, void* stream) {
+  g_err[0] = 0;
+  if (int rc = check_window(cache, true)) return rc;
+  if (n_tokens < 0 || n_tokens > 0x7fffffff) return fail(KVM_ERR_BAD_ARGUMENT, "n_tokens %lld outside [0, 2^31)", (long long)n_tokens);
+  if (n_tokens == 0) return KVM_OK;
+  if (int rc = check_tensor(k, "k", cache->head_dim)) return rc;
+  if (int rc = check_tensor(v, "v", cache->head_dim)) return rc;
+  if (!positions_dev && (int64_t)position + n_tokens > 0x7fffffff)
+    return fail(KVM_ERR_BAD_ARGUMENT, "position %d: tokens beyond 2^31 - 1", position);
+  const cudaError_t e = window_write_dispatch(cache->head_dim, cache->bits, window_dev(cache), to_dev(k), to_dev(v), (int)n_tokens,
+                                              SeqInts{positions_dev, position}, SeqInts{lengths_dev, length},
+                                              static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kvm_window_cache_write");
+  return KVM_OK;
+}
+
+int kvm_window_cache_read(const kvm_window_cache* cache, const int32_t* lengths_dev, int32_t length, void* k_out, void* v_out, void* stream) {
+  g_err[0] = 0;
+  if (int rc = check_window(cache, true)) return rc;
+  if (!k_out || !v_out || ((uintptr_t)k_out) % 16 || ((uintptr_t)v_out) % 16)
+    return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_cache_read: outputs must be 16-byte aligned and not NULL");
+  const cudaError_t e = window_read_dispatch(cache->head_dim, cache->bits, window_dev(cache), SeqInts{lengths_dev, length},
+                                             static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kvm_window_cache_read");
+  return KVM_OK;
+}
+
+int kvm_window_attend(const kvm_window_cache* cache, int32_t n_q_heads, kvm_tensor4 q, kvm_tensor4 k_new, kvm_tensor4 v_new,
+                      const int32_t* lengths_dev, int32_t length, float scale, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  g_err[0] = 0;
+  if (int rc = check_window(cache, true)) return rc;
+  if (int rc = check_groups(cache, n_q_heads)) return rc;
+  if (int rc = check_tensor(q, "q", cache->head_dim)) return rc;
+  if ((k_new.ptr == nullptr) != (v_new.ptr == nullptr)) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: k and v of the new token go together");
+  if (k_new.ptr) {
+    if (int rc = check_tensor(k_new, "k", cache->head_dim)) return rc;
+    if (int rc = check_tensor(v_new, "v", cache->head_dim)) return rc;
+  }
+  if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: out must be 16-byte aligned and not NULL");
+  const int G = n_q_heads / cache->n_kv_heads;
+  if (!workspace || ((uintptr_t)workspace) % 16 || workspace_bytes < window_token_workspace(cache->head_dim, G))
+    return fail(KVM_ERR_CAPACITY, "kvm_window_attend: workspace of %zu bytes (needs %zu, 16-byte aligned)", workspace_bytes,
+                window_token_workspace(cache->head_dim, G));
+  int* status = nullptr;
+  if (int rc = window_status_word(&status)) return rc;
+  const cudaError_t e = window_token_dispatch(cache->head_dim, cache->bits, window_dev(cache), G, to_dev(q), to_dev(k_new), to_dev(v_new),
+                                              SeqInts{lengths_dev, length}, scale, static_cast<float*>(workspace),
+                                              static_cast<bf16*>(out), status, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kvm_window_attend");
+  return KVM_OK;
+}
+
+int kvm_window_attention(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_queries, int64_t n_keys,
+                         kvm_tensor4 q, kvm_tensor4 k, kvm_tensor4 v, int64_t window, int64_t sinks, float scale,
+                         const int32_t* lengths_dev, void* out, void* stream) {
+  g_err[0] = 0;
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128) return fail(KVM_ERR_UNSUPPORTED, "head_dim %d not supported (32, 64 or 128)", head_dim);
+  if (n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
+    return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, n_kv_heads);
+  if (batch < 0 || n_queries < 0 || n_keys < n_queries || n_keys > 0x3fffffff)
+    return fail(KVM_ERR_BAD_ARGUMENT, "batch %d, %lld queries, %lld keys: none negative, at least as many keys as queries, below 2^30", batch,
+                (long long)n_queries, (long long)n_keys);
+  if (window < 1 || sinks < 0) return fail(KVM_ERR_BAD_ARGUMENT, "window %lld must be at least 1, sinks %lld not negative", (long long)window, (long long)sinks);
+  if (batch == 0 || n_queries == 0) return KVM_OK;
+  if (int rc = check_tensor(q, "q", head_dim)) return rc;
+  if (int rc = check_tensor(k, "k", head_dim)) return rc;
+  if (int rc = check_tensor(v, "v", head_dim)) return rc;
+  if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must be 16-byte aligned and not NULL");
+  int* status = nullptr;
+  if (int rc = window_status_word(&status)) return rc;
+  const int w = (int)(window < n_keys ? window : n_keys), s = (int)(sinks < n_keys ? sinks : n_keys);
+  const cudaError_t e = window_prompt_dispatch(head_dim, batch, n_q_heads, n_kv_heads, (int)n_queries, (int)n_keys, to_dev(q), to_dev(k),
+                                               to_dev(v), w, s, scale, lengths_dev, static_cast<bf16*>(out), status,
+                                               static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kvm_window_attention");
+  return KVM_OK;
+}
+
+int kvm_window_status(void* stream) {
+  g_err[0] = 0;
+  int* word = nullptr;
+  if (int rc = window_status_word(&word)) return rc;
+  int st = 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(&st, word, sizeof(int), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && st != 0) e = cudaMemsetAsync(word, 0, sizeof(int), s);  // reported once
+  if (e != cudaSuccess) return cuda_fail(e, "kvm_window_status");
+  if (st == KVM_ERR_DEVICE_TIMEOUT) return fail(st, "a bounded wait inside a window kernel expired (device-side timeout)");
+  if (st != 0) return fail(st, "a window kernel reported status %d", st);
+  return KVM_OK;
 }
 
 int kvm_prefill_workspace_layout(const kvm_layer* layer, int32_t batch, int64_t seq_len, int64_t total_version_rows,
