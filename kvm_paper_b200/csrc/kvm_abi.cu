@@ -262,6 +262,11 @@ int check_window(const kvm_window_cache* c, bool arrays) {
   return KVM_OK;
 }
 
+int check_scale(float scale) {
+  if (!(scale > 0.f && scale < 3e38f)) return fail(KVM_ERR_BAD_ARGUMENT, "scale %g must be positive and finite", (double)scale);
+  return KVM_OK;
+}
+
 int check_groups(const kvm_window_cache* c, int n_q_heads) {
   if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads)
     return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, c->n_kv_heads);
@@ -573,6 +578,7 @@ int kvm_window_attend(const kvm_window_cache* cache, int32_t n_q_heads, kvm_tens
     if (int rc = check_tensor(k_new, "k", cache->head_dim)) return rc;
     if (int rc = check_tensor(v_new, "v", cache->head_dim)) return rc;
   }
+  if (int rc = check_scale(scale)) return rc;
   if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: out must be 16-byte aligned and not NULL");
   const int G = n_q_heads / cache->n_kv_heads;
   if (!workspace || ((uintptr_t)workspace) % 16 || workspace_bytes < window_token_workspace(cache->head_dim, G))
@@ -602,6 +608,13 @@ int kvm_window_attention(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, i
   if (int rc = check_tensor(q, "q", head_dim)) return rc;
   if (int rc = check_tensor(k, "k", head_dim)) return rc;
   if (int rc = check_tensor(v, "v", head_dim)) return rc;
+  if (int rc = check_scale(scale)) return rc;
+  // (the copies step by the strides: an expanded dimension is the caller's to lay out)
+  const kvm_tensor4* in[3] = {&q, &k, &v};
+  for (int i = 0; i < 3; ++i)
+    if ((batch > 1 && in[i]->stride_b <= 0) || ((i ? n_kv_heads : n_q_heads) > 1 && in[i]->stride_h <= 0) ||
+        ((i ? n_keys : n_queries) > 1 && in[i]->stride_t <= 0))
+      return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: strides must be positive");
   if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must be 16-byte aligned and not NULL");
   int* status = nullptr;
   if (int rc = window_status_word(&status)) return rc;

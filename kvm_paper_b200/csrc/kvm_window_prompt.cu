@@ -1,70 +1,522 @@
 // Attention of a prompt, or of a chunk of one behind earlier tokens, with a sliding window and sinks: query t stands at
-// position S - T + t and sees position j if j <= p and (j > p - window or j < sinks).
+// position S - T + t and sees position j if j <= p and (j > p - window or j < sinks).  tcgen05 + tensor memory.
+//
+// One persistent CTA per SM; a work item is two query tiles of 128 rows that share their key and value tiles of 128 rows:
+// two query heads of one kv head over the same queries where the heads per kv head are even in number, else 256 queries of
+// one head.  The tiles of an item: those of the sinks that lie before the window, then the window's, from the first key that
+// the item's first query sees to its last query.
+//
+//   producer (1 warp)      one thread: tiled TMA copies of the query tiles and, through a ring of slots, of K0, V0, K1, ...
+//   MMA (1 warp per tile)  one thread: S = Q K^T into tensor memory; O += P V with P as the tensor-memory A operand, in two
+//                          halves of 64 keys as the softmax delivers them.  P lies over the scores it came from, so the next
+//                          scores follow behind P V; while one tile is in its softmax the other has the tensor core.
+//   softmax (4 warps per tile)  one query row per thread: scores from tensor memory, mask (only where a tile is not seen
+//                          whole), running maximum (raised, and O rescaled, when a tile exceeds it by 2^8), exp2, row sum
+//                          (fp32), P as bf16; behind the last tile O / l to global memory.
+// Infinities and NaN in values that a row does not see: a masked weight is 0, and 0 x inf would reach the row through the
+// product.  Value rows behind a sequence's length are cleared in shared memory; for any other, a row whose sum is finite
+// but whose output is not is computed again by its thread from the keys that it sees (redo_row).
+// Every wait is bounded; one that runs out sets the status word, and the CTA leaves through its common exit.
+#include <algorithm>
+
+#include "kvm_tma_host.cuh"
 #include "kvm_window.cuh"
 
 namespace kvm {
 
 namespace {
 
-// One warp per (sequence, query head, query): lanes take one key each, then D/32 channels each.
-template <int D>
-__global__ void __launch_bounds__(256)
-kvm_window_prompt_kernel(int Hq, int Hkv, int T, int S, Tensor4 q, Tensor4 k, Tensor4 v, int window, int sinks, float scale_log2,
-                         const int* __restrict__ lengths, bf16* __restrict__ out) {
-  constexpr int CPL = D / 32;
-  __shared__ float qs[8][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * 8 + warp, hq = blockIdx.y % Hq, b = blockIdx.y / Hq, h = hq / (Hq / Hkv);
-  if (t >= T) return;
-  const int p = S - T + t;
-  bf16* dst = out + ((size_t)b * T + t) * Hq * D + (size_t)hq * D + lane * CPL;
-  float o[CPL], m = -INFINITY, l = 0.f;
+constexpr int kRows = 128;   // queries per tile, keys per tile
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kRegsSoftmax = 224, kRegsOther = 56, kRegsLaunch = 168;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split above the block's registers");
+
+// DP: head dimension as the tiles hold it (64 or 128; one of 32 is padded with zeros by the copies)
+template <int DP>
+struct PC {
+  static constexpr int kTileBytes = kRows * DP * 2;
+  static constexpr int kSlots = DP == 128 ? 5 : 8;
+  static constexpr int kOffKv = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffKv + kSlots * kTileBytes;
+  static constexpr int kSmem = kOffBar + 512;
+  static constexpr uint32_t kColO = 256;  // first column of the outputs; scores of tile i in columns 128 i ..
+};
+
+struct PromptBars {
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], pv_done[2], o_final[2], o_free[2];
+  uint32_t tmem_base;
+};
+
+struct PromptArgs {
+  int B, Hq, Hkv, D, T, S, window, sinks, pair_heads, n_items, units, q_tiles;  // units: (sequence, head or head pair)
+  float scale_log2;
+  const int* lengths;
+  bf16* out;
+  int* status;
+  Tensor4 q, k, v;
+  CUtensorMap mq, mk, mv;
+  int q_head_inner, k_head_inner, v_head_inner;
+};
+
+// What an item is, computed alike by every role.
+struct Item {
+  int b, hkv, len, lo, s_end, n_sink, n_tiles;  // first window key, end of the sinks before it, their tiles, tiles in all
+  int hq[2], t0[2], begin[2], end[2];           // per query tile: head, first query, window tiles [begin, end) in list places
+  __device__ __forceinline__ Item(const PromptArgs& a, int x) {
+    const int qt = a.q_tiles - 1 - x / a.units, u = x % a.units;  // (later, heavier tiles first)
+    const int per_seq = a.units / a.B, G = a.Hq / a.Hkv;
+    b = u / per_seq;
+    const int hu = u % per_seq;
+    if (a.pair_heads) {
+      hq[0] = hu * 2;
+      hq[1] = hq[0] + 1;
+      t0[0] = t0[1] = qt * kRows;
+    } else {
+      hq[0] = hq[1] = hu;
+      t0[0] = qt * 2 * kRows;
+      t0[1] = t0[0] + kRows;
+    }
+    hkv = hq[0] / G;
+    len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+    const int at = a.S - a.T;
+    lo = max(0, at + t0[0] - a.window + 1);
+    int hi_all = 0;
+    s_end = min(a.sinks, lo);
+    n_sink = (s_end + kRows - 1) / kRows;
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) o[i] = 0.f;
-  if (!lengths || p < lengths[b]) {
-    for (int i = lane; i < D; i += 32) qs[warp][i] = __bfloat162float(q.row(b, hq, t)[i]) * scale_log2;
-    __syncwarp();
-    const int lo = max(0, p - window + 1), ns = min(sinks, lo);
-    for (int base = 0; base < ns + p + 1 - lo; base += 32) {
-      const int i = base + lane, j = i < ns ? i : lo + i - ns;
-      float s = -INFINITY;
-      if (j <= p) {
-        s = 0.f;
-        const bf16* kr = k.row(b, h, j);
-        for (int d = 0; d < D; ++d) s = fmaf(qs[warp][d], __bfloat162float(kr[d]), s);
+    for (int i = 0; i < 2; ++i) {
+      const int p0 = at + t0[i], hi = min(min(at + a.T, p0 + kRows), len);  // first query's position, end of the seen keys
+      begin[i] = end[i] = 0;
+      if (t0[i] < a.T && p0 < len) {
+        // (sinks inside the window's tiles: from its first one on)
+        const int lo_i = a.sinks > lo ? lo : max(lo, p0 - a.window + 1);
+        begin[i] = n_sink + (lo_i - lo) / kRows;
+        end[i] = n_sink + (hi - lo + kRows - 1) / kRows;
       }
-      const float mn = fmaxf(m, warp_max(s)), mm = mn == -INFINITY ? 0.f : mn, a = exp2f(m - mm), e = exp2f(s - mm);
-      l = l * a + warp_sum(e);
-      m = mn;
+      hi_all = max(hi_all, end[i]);
+    }
+    n_tiles = hi_all;
+  }
+  __device__ __forceinline__ int key0(int u) const { return u < n_sink ? u * kRows : lo + (u - n_sink) * kRows; }
+  template <int I>
+  __device__ __forceinline__ bool uses(int u) const { return u < n_sink ? end[I] > 0 : u >= begin[I] && u < end[I]; }
+  template <int I>
+  __device__ __forceinline__ int count() const { return end[I] > 0 ? n_sink + end[I] - begin[I] : 0; }
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity)); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* m, bool head_inner, int x, int t, int h, int b, uint64_t* bar) {
+  if (head_inner) tc::tma_load_4d(dst, m, x, h, t, b, bar);
+  else tc::tma_load_4d(dst, m, x, t, h, b, bar);
+}
+template <int DP>
+__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* m, bool head_inner, int t, int h, int b, uint64_t* bar) {
+  tc::mbar_arrive_expect_tx(bar, PC<DP>::kTileBytes);
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) o[c] *= a;
-      for (int x = 0; x < 32; ++x) {
-        const float w = __shfl_sync(0xffffffffu, e, x);
-        const int jx = __shfl_sync(0xffffffffu, j, x);
-        if (jx > p) break;
-        const bf16* vr = v.row(b, h, jx) + lane * CPL;
+  for (int x = 0; x < DP; x += 64) load_box(dst + x * kRows * 2, m, head_inner, x, t, h, b, bar);
+}
+
+// ------------------------------------------------------------------------------------------ producer
+template <int DP>
+__device__ __forceinline__ bool produce(const PromptArgs& a, unsigned char* smem, PromptBars* bars) {
+  int slot = 0, round = 0;  // of the ring
+  auto kv = [&](const CUtensorMap* m, bool hi, int key, const Item& it) {
+    if (round > 0 && !tc::mbar_wait(&bars->kv_empty[slot], (round - 1) & 1)) return false;
+    load_tile<DP>(smem + PC<DP>::kOffKv + slot * PC<DP>::kTileBytes, m, hi, key, it.hkv, it.b, &bars->kv_full[slot]);
+    if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
+    return true;
+  };
+  int nq[2] = {0, 0};
+  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
+    const Item it(a, x);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) o[c] = fmaf(w, __bfloat162float(vr[c]), o[c]);
+    for (int i = 0; i < 2; ++i) {
+      if (it.end[i] == 0) continue;
+      if (nq[i] > 0 && !tc::mbar_wait(&bars->q_empty[i], (nq[i] - 1) & 1)) return false;
+      load_tile<DP>(smem + i * PC<DP>::kTileBytes, &a.mq, a.q_head_inner, it.t0[i], it.hq[i], it.b, &bars->q_full[i]);
+      ++nq[i];
+    }
+    for (int u = 0; u < it.n_tiles; ++u) {
+      if (!kv(&a.mk, a.k_head_inner, it.key0(u), it)) return false;
+      if (!kv(&a.mv, a.v_head_inner, it.key0(u), it)) return false;
+    }
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------------------------------ MMA issue
+template <int DP, int I>
+__device__ __forceinline__ bool issue(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem) {
+  constexpr uint32_t idesc_qk = tc::make_idesc(kRows, kRows, 0, 0), idesc_pv = tc::make_idesc(kRows, DP, 0, 1);
+  const uint64_t dq = tc::make_desc(tc::smem_u32(smem + I * PC<DP>::kTileBytes), 16, 1024);
+  const uint64_t dk0 = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
+  const uint64_t dv0 = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);
+  const uint32_t col_s = tmem + I * 128, col_o = tmem + PC<DP>::kColO + I * DP;
+  int slot = 0, round = 0, n = 0, nq = 0;  // ring place of the next tile, tiles and items of this query tile so far
+  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
+    const Item it(a, x);
+    const int cnt = it.count<I>();
+    if (cnt > 0) {
+      if (!tc::mbar_wait(&bars->q_full[I], nq & 1)) return false;
+      ++nq;
+    }
+    int done = 0;
+    for (int u = 0; u < it.n_tiles; ++u) {
+      const int ks = slot, kr = round & 1;
+      if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
+      const int vs = slot, vr = round & 1;
+      if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
+      if (!tc::mbar_wait(&bars->kv_full[ks], kr)) return false;
+      if (!it.uses<I>(u)) {  // arrivals stay in step with the slots' uses
+        tc::mbar_arrive(&bars->kv_empty[ks]);
+        if (!tc::mbar_wait(&bars->kv_full[vs], vr)) return false;
+        tc::mbar_arrive(&bars->kv_empty[vs]);
+        continue;
+      }
+      tc::tc_fence_after_sync();
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const uint64_t off = (uint64_t)(((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4);
+        tc::mma_ss(col_s, dq + off, dk0 + (uint64_t)((ks * PC<DP>::kTileBytes) >> 4) + off, idesc_qk, s > 0);
+      }
+      tc::mma_commit(&bars->s_full[I]);
+      tc::mma_commit(&bars->kv_empty[ks]);
+      ++done;
+      if (done == cnt) tc::mma_commit(&bars->q_empty[I]);
+      if (done == 1 && nq > 1 && !tc::mbar_wait(&bars->o_free[I], (nq - 2) & 1)) return false;  // the last item's output has been read
+      if (!tc::mbar_wait(&bars->kv_full[vs], vr)) return false;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!tc::mbar_wait(&bars->p_full[I][half], n & 1)) return false;
+        tc::tc_fence_after_sync();
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          tc::mma_ts(col_o, col_s + (half * 4 + s) * 8, dv0 + (uint64_t)((vs * PC<DP>::kTileBytes + (half * 4 + s) * 2048) >> 4), idesc_pv,
+                     done > 1 || half > 0 || s > 0);
+      }
+      tc::mma_commit(&bars->pv_done[I]);
+      tc::mma_commit(&bars->kv_empty[vs]);
+      if (done == cnt) tc::mma_commit(&bars->o_final[I]);
+      ++n;
+    }
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------------------------------ softmax
+// One query row of which a value that it does not see was an infinity or NaN: the weighted sum over the keys that it sees,
+// with the maximum and the sum that the tiles gave (the weights are not rounded here).
+__device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hkv, int t, int p, float m, float inv) {
+  const bf16* qr = a.q.row(b, hq, t);
+  bf16* dst = a.out + (((size_t)b * a.T + t) * a.Hq + hq) * a.D;
+  const int lo = max(0, p - a.window + 1), ns = min(a.sinks, lo);
+  const float neg_m = m == -INFINITY ? 0.f : -m;
+  for (int c0 = 0; c0 < a.D; c0 += 32) {
+    float acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < ns + p + 1 - lo; ++i) {
+      const int j = i < ns ? i : lo + i - ns;
+      const bf16* kr = a.k.row(b, hkv, j);
+      float s = 0.f;
+      for (int d = 0; d < a.D; d += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(qr + d), y = *reinterpret_cast<const uint4*>(kr + d);
+        const unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16(xs[e]), h = unpack_bf16(ys[e]);
+          s = fmaf(f.x, h.x, fmaf(f.y, h.y, s));
+        }
+      }
+      const float w = ex2(fmaf(s, a.scale_log2, neg_m));
+      const bf16* vr = a.v.row(b, hkv, j) + c0;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        const uint4 y = *reinterpret_cast<const uint4*>(vr + e);
+        const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float2 h = unpack_bf16(ys[z]);
+          acc[e + 2 * z] = fmaf(w, h.x, acc[e + 2 * z]);
+          acc[e + 2 * z + 1] = fmaf(w, h.y, acc[e + 2 * z + 1]);
+        }
       }
     }
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) o[c] /= l;
+    for (int e = 0; e < 32; e += 2) *reinterpret_cast<uint32_t*>(dst + c0 + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
   }
+}
+
+template <int DP, int I>
+__device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem, int row, int wq, int lane) {
+  const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
+  const uint32_t col_s = lane_addr + I * 128, col_o = lane_addr + PC<DP>::kColO + I * DP;
+  const float sc = a.scale_log2;
+  int slot = 0, round = 0, n = 0, ni = 0;
+  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
+    const Item it(a, x);
+    const int t = it.t0[I] + row, p0 = a.S - a.T + it.t0[I], p = p0 + row;
+    float m_run = -INFINITY, l_run = 0.f;
+    int done = 0;
+    for (int u = 0; u < it.n_tiles; ++u) {
+      if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }  // (the keys' slot)
+      const int vs = slot, vr = round & 1;
+      if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
+      if (!it.uses<I>(u)) continue;
+      const int key0 = it.key0(u);
+      if (!warp_wait(&bars->s_full[I], n & 1)) return false;
+      tc::tc_fence_after_sync();
+      uint32_t sr[4][32];
 #pragma unroll
-  for (int c = 0; c < CPL; ++c) dst[c] = __float2bfloat16_rn(o[c]);
+      for (int c = 0; c < 4; ++c) tc::tmem_ld32(col_s + c * 32, sr[c]);
+      tc::tmem_ld_wait();
+      // is the tile seen whole by all rows?
+      const bool sink_tile = u < it.n_sink;
+      const bool whole = sink_tile ? key0 + kRows <= it.s_end : key0 + kRows - 1 <= p0 && (key0 > p0 + kRows - 1 - a.window || key0 + kRows <= a.sinks);
+      if (!whole) {
+        // columns [c_lo, c_hi) and those below c_s are seen
+        const int c_hi = sink_tile ? it.s_end - key0 : p + 1 - key0, c_lo = sink_tile ? 0 : p - a.window + 1 - key0;
+        const int c_s = sink_tile ? 0 : a.sinks - key0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          auto below = [](int k) { return k <= 0 ? 0u : (k >= 32 ? 0xffffffffu : (1u << k) - 1u); };
+          const unsigned hi = below(c_hi - c * 32), seen = (hi & ~below(c_lo - c * 32)) | (hi & below(c_s - c * 32));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((seen >> i) & 1u)) sr[c][i] = 0xff800000u;  // -inf
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+      }
+      const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+      const bool need = tmax > m_run + kRescale || (m_run == -INFINITY && tmax > -INFINITY);
+      if (__any_sync(0xffffffffu, need)) {
+        const float m_new = need ? tmax : m_run;
+        const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - m_new);
+        if (done > 0) {  // O may only be touched between P V of the last tile (complete) and of this one (waits for this warp)
+          if (!warp_wait(&bars->pv_done[I], (n - 1) & 1)) return false;
+          tc::tc_fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tc::tmem_ld16(col_o + c, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tc::tmem_st16(col_o + c, o);
+          }
+          tc::tmem_st_wait();
+        }
+        l_run *= alpha;
+        m_run = m_new;
+      }
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
+      float2 ls = make_float2(0.f, 0.f);
+      // value rows behind the sequence's length: padding, cleared before the product reads them
+      if (it.len < a.S && key0 + kRows > it.len) {
+        if (!warp_wait(&bars->kv_full[vs], vr)) return false;
+        if (key0 + row >= it.len) {
+          unsigned char* vrow = smem + PC<DP>::kOffKv + vs * PC<DP>::kTileBytes + row * 128;
+#pragma unroll
+          for (int c = 0; c < DP / 8; ++c) *reinterpret_cast<uint4*>(vrow + (c >> 3) * (kRows * 128) + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        tc::fence_proxy_async();
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t* s2 = &sr[half * 2 + c][e * 2];
+            const float2 z = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])), sc2, nm2);
+            const float2 w = make_float2(ex2(z.x), ex2(z.y));
+            ls = __fadd2_rn(ls, w);
+            pk[e] = pack_bf16(w.x, w.y);
+          }
+          tc::tmem_st16(col_s + (half * 2 + c) * 16, pk);
+        }
+        tc::tmem_st_wait();
+        tc::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars->p_full[I][half]);
+      }
+      l_run += ls.x + ls.y;
+      ++done;
+      ++n;
+    }
+    // ---- the item's output
+    bf16* dst = a.out + (((size_t)it.b * a.T + t) * a.Hq + it.hq[I]) * a.D;
+    const bool mine = t < a.T;
+    if (done == 0) {
+      if (mine)
+        for (int c = 0; c < a.D; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    if (!warp_wait(&bars->o_final[I], ni & 1)) return false;
+    ++ni;
+    tc::tc_fence_after_sync();
+    const bool valid = mine && p < it.len;
+    const float inv = valid ? 1.0f / l_run : 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int hb = 0; hb < DP / 32; ++hb) {
+      uint32_t o[32];
+      tc::tmem_ld32(col_o + hb * 32, o);
+      tc::tmem_ld_wait();
+      if (hb * 32 < a.D && mine) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          bad |= !(fabsf(__uint_as_float(o[i])) < INFINITY);
+          o[i] = valid ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          uint4 y;
+          y.x = pack_bf16(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+          y.y = pack_bf16(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+          y.z = pack_bf16(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
+          y.w = pack_bf16(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+          *reinterpret_cast<uint4*>(dst + hb * 32 + i) = y;
+        }
+      }
+    }
+    tc::tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&bars->o_free[I]);
+    if (bad && valid && l_run < INFINITY) redo_row(a, it.b, it.hq[I], it.hkv, t, p, m_run, inv);
+    __syncwarp();
+  }
+  return true;
+}
+
+}  // namespace
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __grid_constant__ PromptArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  PromptBars* bars = reinterpret_cast<PromptBars*>(smem + PC<DP>::kOffBar);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if ((tc::smem_u32(smem) & 1023u) != 0) {  // operand tiles need 1024-byte alignment
+    if (tid == 0) atomicExch(a.status, KVM_ERR_UNSUPPORTED);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars->q_full[i], 1);
+      tc::mbar_init(&bars->q_empty[i], 1);
+      tc::mbar_init(&bars->s_full[i], 1);
+      tc::mbar_init(&bars->p_full[i][0], 4);
+      tc::mbar_init(&bars->p_full[i][1], 4);
+      tc::mbar_init(&bars->pv_done[i], 1);
+      tc::mbar_init(&bars->o_final[i], 1);
+      tc::mbar_init(&bars->o_free[i], 4);
+    }
+    for (int i = 0; i < PC<DP>::kSlots; ++i) {
+      tc::mbar_init(&bars->kv_full[i], 1);
+      tc::mbar_init(&bars->kv_empty[i], 2);
+    }
+    tc::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(&bars->tmem_base, 512);
+  pdl_wait();
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  tc::tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  bool ok = true;
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    ok = warp < 4 ? softmax<DP, 0>(a, smem, bars, tmem, tid & 127, warp & 3, lane) : softmax<DP, 1>(a, smem, bars, tmem, tid & 127, warp & 3, lane);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (lane == 0) {
+      if (warp == kProducerWarp) ok = produce<DP>(a, smem, bars);
+      else if (warp == kMmaWarp) ok = issue<DP, 0>(a, smem, bars, tmem);
+      else if (warp == kMmaWarp + 1) ok = issue<DP, 1>(a, smem, bars, tmem);
+    }
+    __syncwarp();
+  }
+  if (!ok) {
+    atomicExch(a.status, KVM_ERR_DEVICE_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies and products in flight
+  }
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+namespace {
+
+// [batch][head][row][D] with any strides as a 4-D tensor, boxes of 64 elements x 128 rows; dimensions ordered by stride
+bool encode_rows(CUtensorMap* m, const Tensor4& t, int batch, int heads, int rows, int D, int* head_inner) {
+  *head_inner = t.sh < t.st && heads > 1;
+  auto bytes = [&](long long s, int n) { return (cuuint64_t)(n > 1 ? s * 2 : (long long)D * 2); };  // (one entry: never stepped over)
+  const cuuint64_t sh = bytes(t.sh, heads), st = bytes(t.st, rows), sb = bytes(t.sb, batch);
+  if (*head_inner) {
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)batch}, strides[3] = {sh, st, sb};
+    const cuuint32_t box[4] = {64, 1, kRows, 1};
+    return encode_bf16_map(m, t.ptr, 4, dims, strides, box);
+  }
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch}, strides[3] = {st, sh, sb};
+  const cuuint32_t box[4] = {64, kRows, 1, 1};
+  return encode_bf16_map(m, t.ptr, 4, dims, strides, box);
+}
+
+template <int DP>
+cudaError_t launch_prompt(const PromptArgs& a, int sms, cudaStream_t stream) {
+  auto kern = kvm_window_prompt_kernel<DP>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PC<DP>::kSmem);
+  if (e != cudaSuccess) return e;
+  // the register split draws on what the block is launched with
+  static const bool regs_ok = [&] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, kern) == cudaSuccess && at.numRegs == kRegsLaunch;
+  }();
+  if (!regs_ok) return cudaErrorInvalidConfiguration;
+  return launch_pdl(kern, dim3(std::min(a.n_items, sms)), dim3(kThreads), PC<DP>::kSmem, stream, true, a);
 }
 
 }  // namespace
 
 cudaError_t window_prompt_dispatch(int D, int batch, int Hq, int Hkv, int T, int S, Tensor4 q, Tensor4 k, Tensor4 v, int window,
                                    int sinks, float scale, const int* lengths, bf16* out, int* status, cudaStream_t stream) {
-  (void)status;
-  const dim3 grid((T + 7) / 8, batch * Hq);
-  auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream>>>(Hq, Hkv, T, S, q, k, v, window, sinks, scale * kLog2e, lengths, out);
-    return cudaGetLastError();
-  };
-  return D == 128 ? go(kvm_window_prompt_kernel<128>) : D == 64 ? go(kvm_window_prompt_kernel<64>) : go(kvm_window_prompt_kernel<32>);
+  PromptArgs a;
+  a.B = batch; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.T = T; a.S = S; a.window = window; a.sinks = sinks;
+  a.scale_log2 = scale * kLog2e;
+  a.lengths = lengths; a.out = out; a.status = status;
+  a.q = q; a.k = k; a.v = v;
+  a.pair_heads = (Hq / Hkv) % 2 == 0;
+  const int rows = a.pair_heads ? kRows : 2 * kRows;
+  a.q_tiles = (T + rows - 1) / rows;
+  const long long units = (long long)batch * (a.pair_heads ? Hq / 2 : Hq);
+  if (units * a.q_tiles > 0x3fffffff) return cudaErrorInvalidValue;
+  a.units = (int)units;
+  a.n_items = (int)units * a.q_tiles;
+  if (!encode_rows(&a.mq, q, batch, Hq, T, D, &a.q_head_inner) || !encode_rows(&a.mk, k, batch, Hkv, S, D, &a.k_head_inner) ||
+      !encode_rows(&a.mv, v, batch, Hkv, S, D, &a.v_head_inner))
+    return cudaErrorInvalidValue;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+  return D == 128 ? launch_prompt<128>(a, sms, stream) : launch_prompt<64>(a, sms, stream);
 }
 
 }  // namespace kvm

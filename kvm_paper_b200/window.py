@@ -43,7 +43,7 @@ def _rows(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
         raise ValueError("the window operators implement inference only; call them under torch.no_grad()")
     st = t.stride()
     # (a dimension of one entry is never stepped over)
-    if st[3] != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for s, n in zip(st[:3], t.shape) if n > 1):
+    if st[3] != 1 or t.data_ptr() % 16 or any(s % 8 or s <= 0 for s, n in zip(st[:3], t.shape) if n > 1):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -77,8 +77,8 @@ def _output(out, shape, dev) -> torch.Tensor:
 
 def _scale(scale, head_dim: int) -> float:
     s = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not math.isfinite(s):
-        raise ValueError(f"scale must be finite, got {s}")
+    if not 0.0 < s < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {s}")
     return s
 
 
