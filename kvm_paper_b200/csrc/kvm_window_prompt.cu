@@ -7,7 +7,7 @@
 // the item's first query sees to its last query.
 //
 //   producer (1 warp)      one thread: tiled TMA copies of the query tiles and, through a ring of slots, of K0, V0, K1, ...
-//   MMA (1 warp per tile)  one thread: S = Q K^T into tensor memory; O += P V with P as the tensor-memory A operand, in two
+//   MMA (1 warp)           one thread: S = Q K^T into tensor memory; O += P V with P as the tensor-memory A operand, in two
 //                          halves of 64 keys as the softmax delivers them.  P lies over the scores it came from, so the next
 //                          scores follow behind P V; while one tile is in its softmax the other has the tensor core.
 //   softmax (4 warps per tile)  one query row per thread: scores from tensor memory, mask (only where a tile is not seen
@@ -30,7 +30,7 @@ constexpr int kRows = 128;   // queries per tile, keys per tile
 constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr float kRescale = 8.0f;  // log2 units
-constexpr int kRegsSoftmax = 224, kRegsOther = 56, kRegsLaunch = 168;
+constexpr int kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split above the block's registers");
 
 // DP: head dimension as the tiles hold it (64 or 128; one of 32 is padded with zeros by the copies)
@@ -100,13 +100,26 @@ struct Item {
     n_tiles = hi_all;
   }
   __device__ __forceinline__ int key0(int u) const { return u < n_sink ? u * kRows : lo + (u - n_sink) * kRows; }
-  template <int I>
-  __device__ __forceinline__ bool uses(int u) const { return u < n_sink ? end[I] > 0 : u >= begin[I] && u < end[I]; }
-  template <int I>
-  __device__ __forceinline__ int count() const { return end[I] > 0 ? n_sink + end[I] - begin[I] : 0; }
+  // (i: 0 or 1; picked so that the item stays in registers)
+  __device__ __forceinline__ int pick(const int (&x)[2], int i) const { return i ? x[1] : x[0]; }
+  __device__ __forceinline__ bool uses(int i, int u) const { return u < n_sink ? pick(end, i) > 0 : u >= pick(begin, i) && u < pick(end, i); }
+  __device__ __forceinline__ int count(int i) const { return pick(end, i) > 0 ? n_sink + pick(end, i) - pick(begin, i) : 0; }
 };
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity)); }
+// Bounded wait without pauses between the tries: the roles hand tiles to each other several times per microsecond, and a
+// pause that overshoots is on the path of both.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 22); ++i)
+    if (tc::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+// One thread of a converged warp, the same one every time.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -133,7 +146,7 @@ template <int DP>
 __device__ __forceinline__ bool produce(const PromptArgs& a, unsigned char* smem, PromptBars* bars) {
   int slot = 0, round = 0;  // of the ring
   auto kv = [&](const CUtensorMap* m, bool hi, int key, const Item& it) {
-    if (round > 0 && !tc::mbar_wait(&bars->kv_empty[slot], (round - 1) & 1)) return false;
+    if (round > 0 && !wait(&bars->kv_empty[slot], (round - 1) & 1)) return false;
     load_tile<DP>(smem + PC<DP>::kOffKv + slot * PC<DP>::kTileBytes, m, hi, key, it.hkv, it.b, &bars->kv_full[slot]);
     if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
     return true;
@@ -144,7 +157,7 @@ __device__ __forceinline__ bool produce(const PromptArgs& a, unsigned char* smem
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (it.end[i] == 0) continue;
-      if (nq[i] > 0 && !tc::mbar_wait(&bars->q_empty[i], (nq[i] - 1) & 1)) return false;
+      if (nq[i] > 0 && !wait(&bars->q_empty[i], (nq[i] - 1) & 1)) return false;
       load_tile<DP>(smem + i * PC<DP>::kTileBytes, &a.mq, a.q_head_inner, it.t0[i], it.hq[i], it.b, &bars->q_full[i]);
       ++nq[i];
     }
@@ -157,62 +170,112 @@ __device__ __forceinline__ bool produce(const PromptArgs& a, unsigned char* smem
 }
 
 // ------------------------------------------------------------------------------------------ MMA issue
-template <int DP, int I>
+// One thread for both query tiles, so that the products of one tile run as a block (P V of its last tile, then the scores of
+// the next) while the other is in its softmax.  (Two issuing threads interleave on the tensor core: both tiles' scores then
+// come late and together, both softmaxes run at the same time, and the tensor core idles meanwhile.)  Step u: P V of
+// tile u - 1 and Q K of tile u, for query tile 0, then for 1; it goes on from item to item.
+template <int DP>
+struct Issuer {
+  static constexpr uint32_t kIdescQk = tc::make_idesc(kRows, kRows, 0, 0), kIdescPv = tc::make_idesc(kRows, DP, 0, 1);
+  PromptBars* bars;
+  uint64_t dq, dk, dv;
+  uint32_t tmem;
+  int n[2] = {0, 0}, nq[2] = {0, 0};   // tiles whose P V is issued, items begun
+  bool pending[2] = {false, false}, first[2], last[2];
+  int pv_slot = 0, pv_parity = 0;      // value slot of the pending tiles
+  bool slot_held = false;
+
+  template <int I>
+  __device__ __forceinline__ bool pv() {  // of the pending tile
+    if (!pending[I]) return true;
+    pending[I] = false;
+    if (first[I] && nq[I] > 1 && !warp_wait(&bars->o_free[I], (nq[I] - 2) & 1)) return false;  // the last item's output has been read
+    if (!warp_wait(&bars->kv_full[pv_slot], pv_parity)) return false;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (!warp_wait(&bars->p_full[I][half], n[I] & 1)) return false;
+      tc::tc_fence_after_sync();
+      if (elected()) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          tc::mma_ts(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + (half * 4 + s) * 8,
+                     dv + (uint64_t)((pv_slot * PC<DP>::kTileBytes + (half * 4 + s) * 2048) >> 4), kIdescPv, !first[I] || half > 0 || s > 0);
+        if (half == 1) {
+          tc::mma_commit(&bars->pv_done[I]);
+          if (last[I]) tc::mma_commit(&bars->o_final[I]);
+        }
+      }
+      __syncwarp();
+    }
+    ++n[I];
+    return true;
+  }
+  template <int I>
+  __device__ __forceinline__ bool qk(int k_slot, bool is_first, bool is_last) {
+    if (is_first) {
+      if (!warp_wait(&bars->q_full[I], nq[I] & 1)) return false;
+      ++nq[I];
+    }
+    tc::tc_fence_after_sync();
+    if (elected()) {
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const uint64_t off = (uint64_t)(((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4);
+        tc::mma_ss(tmem + I * 128, dq + (uint64_t)((I * PC<DP>::kTileBytes) >> 4) + off, dk + (uint64_t)((k_slot * PC<DP>::kTileBytes) >> 4) + off,
+                   kIdescQk, s > 0);
+      }
+      tc::mma_commit(&bars->s_full[I]);
+      if (is_last) tc::mma_commit(&bars->q_empty[I]);
+    }
+    __syncwarp();
+    pending[I] = true;
+    first[I] = is_first;
+    last[I] = is_last;
+    return true;
+  }
+  __device__ __forceinline__ void commit(uint64_t* bar) {
+    if (elected()) tc::mma_commit(bar);
+    __syncwarp();
+  }
+};
+
+template <int DP>
 __device__ __forceinline__ bool issue(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem) {
-  constexpr uint32_t idesc_qk = tc::make_idesc(kRows, kRows, 0, 0), idesc_pv = tc::make_idesc(kRows, DP, 0, 1);
-  const uint64_t dq = tc::make_desc(tc::smem_u32(smem + I * PC<DP>::kTileBytes), 16, 1024);
-  const uint64_t dk0 = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
-  const uint64_t dv0 = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);
-  const uint32_t col_s = tmem + I * 128, col_o = tmem + PC<DP>::kColO + I * DP;
-  int slot = 0, round = 0, n = 0, nq = 0;  // ring place of the next tile, tiles and items of this query tile so far
+  Issuer<DP> is;
+  is.bars = bars;
+  is.tmem = tmem;
+  is.dq = tc::make_desc(tc::smem_u32(smem), 16, 1024);
+  is.dk = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
+  is.dv = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);
+  int slot = 0, round = 0;
   for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
     const Item it(a, x);
-    const int cnt = it.count<I>();
-    if (cnt > 0) {
-      if (!tc::mbar_wait(&bars->q_full[I], nq & 1)) return false;
-      ++nq;
-    }
-    int done = 0;
+    const int cnt0 = it.count(0), cnt1 = it.count(1);
+    int done0 = 0, done1 = 0;
     for (int u = 0; u < it.n_tiles; ++u) {
       const int ks = slot, kr = round & 1;
       if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
       const int vs = slot, vr = round & 1;
       if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
-      if (!tc::mbar_wait(&bars->kv_full[ks], kr)) return false;
-      if (!it.uses<I>(u)) {  // arrivals stay in step with the slots' uses
-        tc::mbar_arrive(&bars->kv_empty[ks]);
-        if (!tc::mbar_wait(&bars->kv_full[vs], vr)) return false;
-        tc::mbar_arrive(&bars->kv_empty[vs]);
-        continue;
+      if (!warp_wait(&bars->kv_full[ks], kr)) return false;
+      if (!is.template pv<0>()) return false;
+      if (it.uses(0, u)) {
+        ++done0;
+        if (!is.template qk<0>(ks, done0 == 1, done0 == cnt0)) return false;
       }
-      tc::tc_fence_after_sync();
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        const uint64_t off = (uint64_t)(((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4);
-        tc::mma_ss(col_s, dq + off, dk0 + (uint64_t)((ks * PC<DP>::kTileBytes) >> 4) + off, idesc_qk, s > 0);
+      if (!is.template pv<1>()) return false;
+      if (is.slot_held) is.commit(&bars->kv_empty[is.pv_slot]);
+      if (it.uses(1, u)) {
+        ++done1;
+        if (!is.template qk<1>(ks, done1 == 1, done1 == cnt1)) return false;
       }
-      tc::mma_commit(&bars->s_full[I]);
-      tc::mma_commit(&bars->kv_empty[ks]);
-      ++done;
-      if (done == cnt) tc::mma_commit(&bars->q_empty[I]);
-      if (done == 1 && nq > 1 && !tc::mbar_wait(&bars->o_free[I], (nq - 2) & 1)) return false;  // the last item's output has been read
-      if (!tc::mbar_wait(&bars->kv_full[vs], vr)) return false;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (!tc::mbar_wait(&bars->p_full[I][half], n & 1)) return false;
-        tc::tc_fence_after_sync();
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          tc::mma_ts(col_o, col_s + (half * 4 + s) * 8, dv0 + (uint64_t)((vs * PC<DP>::kTileBytes + (half * 4 + s) * 2048) >> 4), idesc_pv,
-                     done > 1 || half > 0 || s > 0);
-      }
-      tc::mma_commit(&bars->pv_done[I]);
-      tc::mma_commit(&bars->kv_empty[vs]);
-      if (done == cnt) tc::mma_commit(&bars->o_final[I]);
-      ++n;
+      is.commit(&bars->kv_empty[ks]);
+      is.pv_slot = vs;
+      is.pv_parity = vr;
+      is.slot_held = true;
     }
   }
-  return true;
+  return is.template pv<0>() && is.template pv<1>();
 }
 
 // ------------------------------------------------------------------------------------------ softmax
@@ -259,22 +322,22 @@ __device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hk
   }
 }
 
-template <int DP, int I>
-__device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem, int row, int wq, int lane) {
+template <int DP>
+__device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem, int I, int row, int wq, int lane) {
   const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
   const uint32_t col_s = lane_addr + I * 128, col_o = lane_addr + PC<DP>::kColO + I * DP;
   const float sc = a.scale_log2;
   int slot = 0, round = 0, n = 0, ni = 0;
   for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
     const Item it(a, x);
-    const int t = it.t0[I] + row, p0 = a.S - a.T + it.t0[I], p = p0 + row;
+    const int t = it.pick(it.t0, I) + row, p0 = a.S - a.T + it.pick(it.t0, I), p = p0 + row;
     float m_run = -INFINITY, l_run = 0.f;
     int done = 0;
     for (int u = 0; u < it.n_tiles; ++u) {
       if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }  // (the keys' slot)
       const int vs = slot, vr = round & 1;
       if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
-      if (!it.uses<I>(u)) continue;
+      if (!it.uses(I, u)) continue;
       const int key0 = it.key0(u);
       if (!warp_wait(&bars->s_full[I], n & 1)) return false;
       tc::tc_fence_after_sync();
@@ -364,7 +427,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
       ++n;
     }
     // ---- the item's output
-    bf16* dst = a.out + (((size_t)it.b * a.T + t) * a.Hq + it.hq[I]) * a.D;
+    bf16* dst = a.out + (((size_t)it.b * a.T + t) * a.Hq + it.pick(it.hq, I)) * a.D;
     const bool mine = t < a.T;
     if (done == 0) {
       if (mine)
@@ -402,7 +465,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
     tc::tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&bars->o_free[I]);
-    if (bad && valid && l_run < INFINITY) redo_row(a, it.b, it.hq[I], it.hkv, t, p, m_run, inv);
+    if (bad && valid && l_run < INFINITY) redo_row(a, it.b, it.pick(it.hq, I), it.hkv, t, p, m_run, inv);
     __syncwarp();
   }
   return true;
@@ -414,7 +477,7 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __grid_constant__ PromptArgs a) {
   extern __shared__ __align__(1024) unsigned char smem[];
   PromptBars* bars = reinterpret_cast<PromptBars*>(smem + PC<DP>::kOffBar);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if ((tc::smem_u32(smem) & 1023u) != 0) {  // operand tiles need 1024-byte alignment
     if (tid == 0) atomicExch(a.status, KVM_ERR_UNSUPPORTED);
     return;
@@ -432,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __
     }
     for (int i = 0; i < PC<DP>::kSlots; ++i) {
       tc::mbar_init(&bars->kv_full[i], 1);
-      tc::mbar_init(&bars->kv_empty[i], 2);
+      tc::mbar_init(&bars->kv_empty[i], 1);
     }
     tc::fence_barrier_init();
   }
@@ -441,19 +504,20 @@ __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __
   tc::tc_fence_before_sync();
   __syncthreads();
   tc::tc_fence_after_sync();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
   bool ok = true;
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    ok = warp < 4 ? softmax<DP, 0>(a, smem, bars, tmem, tid & 127, warp & 3, lane) : softmax<DP, 1>(a, smem, bars, tmem, tid & 127, warp & 3, lane);
+    ok = softmax<DP>(a, smem, bars, tmem, warp >> 2, tid & 127, warp & 3, lane);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (lane == 0) {
-      if (warp == kProducerWarp) ok = produce<DP>(a, smem, bars);
-      else if (warp == kMmaWarp) ok = issue<DP, 0>(a, smem, bars, tmem);
-      else if (warp == kMmaWarp + 1) ok = issue<DP, 1>(a, smem, bars, tmem);
+    if (warp == kProducerWarp) {
+      if (lane == 0) ok = produce<DP>(a, smem, bars);
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // (the whole warp walks the tiles: operands that are uniform over it reach the issuing instructions without detours)
+      ok = issue<DP>(a, smem, bars, tmem);
     }
-    __syncwarp();
   }
   if (!ok) {
     atomicExch(a.status, KVM_ERR_DEVICE_TIMEOUT);
