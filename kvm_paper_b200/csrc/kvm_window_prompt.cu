@@ -8,7 +8,7 @@
 //
 //   producer (1 warp)      one thread: tiled TMA copies of the query tiles and, through a ring of slots, of K0, V0, K1, ...
 //   MMA (1 warp)           one thread: S = Q K^T into tensor memory; O += P V with P as the tensor-memory A operand, in two
-//                          halves of 64 keys as the softmax delivers them.  P lies over the scores it came from, so the next
+//                          parts (96 and 32 keys) as the softmax delivers them.  P lies over the scores it came from, so the next
 //                          scores follow behind P V; while one tile is in its softmax the other has the tensor core.
 //   softmax (4 warps per tile)  one query row per thread: scores from tensor memory, mask (only where a tile is not seen
 //                          whole), running maximum (raised, and O rescaled, when a tile exceeds it by 2^8), exp2, row sum
@@ -18,6 +18,7 @@
 // but whose output is not is computed again by its thread from the keys that it sees (redo_row).
 // Every wait is bounded; one that runs out sets the status word, and the CTA leaves through its common exit.
 #include <algorithm>
+#include <type_traits>
 
 #include "kvm_tma_host.cuh"
 #include "kvm_window.cuh"
@@ -30,6 +31,8 @@ constexpr int kRows = 128;   // queries per tile, keys per tile
 constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kSplit = 3;         // of 4 x 32 keys, those whose weights are handed to the MMA warp first
+constexpr int kPoly = 4;          // of 16 pairs of weights, those formed by polynomial
 constexpr int kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split above the block's registers");
 
@@ -125,10 +128,30 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if any of them is
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {  // clamped to [0, 1]
+  float d;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for two x in [-120, 8], given as y = (x + 120) / 128 (clamping to [0, 1] has clamped x).  Range reduction to the nearest
+// integer and a polynomial of degree 3 on [-1/2, 1/2], minimax in the relative error by Remez exchange: 7.5e-5, a
+// twenty-fifth of the bf16 rounding that follows.  On the FMA pipes: the special-function unit makes 16 exponentials per
+// clock and SM, and both query tiles' softmaxes want 128 x 128 each for every 2048 clocks of the tensor core.
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, which stands in the low bits
+  const float2 t = __ffma2_rn(y, make_float2(128.f, 128.f), make_float2(kMagic - 120.f, kMagic - 120.f));
+  const float2 n = __fadd2_rn(t, make_float2(120.f - kMagic, 120.f - kMagic));  // the integer + 120
+  const float2 f = __ffma2_rn(y, make_float2(128.f, 128.f), make_float2(-n.x, -n.y));
+  float2 p = __ffma2_rn(f, make_float2(0.0551716685295105f, 0.0551716685295105f), make_float2(0.2426111251115799f, 0.2426111251115799f));
+  p = __ffma2_rn(f, p, make_float2(0.6932609677314758f, 0.6932609677314758f));
+  p = __ffma2_rn(f, p, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* m, bool head_inner, int x, int t, int h, int b, uint64_t* bar) {
   if (head_inner) tc::tma_load_4d(dst, m, x, h, t, b, bar);
@@ -197,9 +220,9 @@ struct Issuer {
       tc::tc_fence_after_sync();
       if (elected()) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          tc::mma_ts(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + (half * 4 + s) * 8,
-                     dv + (uint64_t)((pv_slot * PC<DP>::kTileBytes + (half * 4 + s) * 2048) >> 4), kIdescPv, !first[I] || half > 0 || s > 0);
+        for (int s = half * kSplit * 2; s < (half ? 8 : kSplit * 2); ++s)
+          tc::mma_ts(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + s * 8, dv + (uint64_t)((pv_slot * PC<DP>::kTileBytes + s * 2048) >> 4),
+                     kIdescPv, !first[I] || s > 0);
         if (half == 1) {
           tc::mma_commit(&bars->pv_done[I]);
           if (last[I]) tc::mma_commit(&bars->o_final[I]);
@@ -332,6 +355,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
     const Item it(a, x);
     const int t = it.pick(it.t0, I) + row, p0 = a.S - a.T + it.pick(it.t0, I), p = p0 + row;
     float m_run = -INFINITY, l_run = 0.f;
+    bool poison = false;
     int done = 0;
     for (int u = 0; u < it.n_tiles; ++u) {
       if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }  // (the keys' slot)
@@ -368,6 +392,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
         for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
       }
       const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+      poison |= !(tmax < INFINITY);  // NaN or +inf among the scores: the row is NaN
       const bool need = tmax > m_run + kRescale || (m_run == -INFINITY && tmax > -INFINITY);
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? tmax : m_run;
@@ -402,26 +427,39 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
         }
         tc::fence_proxy_async();
       }
+      // weights; where every key is seen, some by polynomial (a masked weight has to be 0, which the polynomial's range
+      // does not hold)
+      const float sc128 = sc * (1.f / 128.f), nm128 = (neg_m + 120.f) * (1.f / 128.f);
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
+          for (int c = half * kSplit; c < (half ? 4 : kSplit); ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t* s2 = &sr[half * 2 + c][e * 2];
-            const float2 z = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])), sc2, nm2);
-            const float2 w = make_float2(ex2(z.x), ex2(z.y));
-            ls = __fadd2_rn(ls, w);
-            pk[e] = pack_bf16(w.x, w.y);
+            for (int e = 0; e < 16; ++e) {
+              const uint32_t* s2 = &sr[c][e * 2];
+              const float s0 = __uint_as_float(s2[0]), s1 = __uint_as_float(s2[1]);
+              float2 w;
+              if (decltype(poly)::value && (e * kPoly) / 16 != ((e + 1) * kPoly) / 16) {  // (spread evenly)
+                w = ex2_fma(make_float2(fma_sat(s0, sc128, nm128), fma_sat(s1, sc128, nm128)));
+              } else {
+                const float2 z = __ffma2_rn(make_float2(s0, s1), sc2, nm2);
+                w = make_float2(ex2(z.x), ex2(z.y));
+              }
+              ls = __fadd2_rn(ls, w);
+              pk[e] = pack_bf16(w.x, w.y);
+            }
+            tc::tmem_st16(col_s + c * 16, pk);
           }
-          tc::tmem_st16(col_s + (half * 2 + c) * 16, pk);
+          tc::tmem_st_wait();
+          tc::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&bars->p_full[I][half]);
         }
-        tc::tmem_st_wait();
-        tc::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bars->p_full[I][half]);
-      }
+      };
+      if (whole) weights(std::true_type{});
+      else weights(std::false_type{});
       l_run += ls.x + ls.y;
       ++done;
       ++n;
@@ -438,6 +476,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
     ++ni;
     tc::tc_fence_after_sync();
     const bool valid = mine && p < it.len;
+    if (poison || m_run == -INFINITY) l_run = __int_as_float(0x7fffffff);  // (no score above -inf: 0 / 0)
     const float inv = valid ? 1.0f / l_run : 0.f;
     bool bad = false;
 #pragma unroll

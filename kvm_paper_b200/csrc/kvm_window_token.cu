@@ -1,15 +1,14 @@
 // Attention of one query per sequence over a window cache (16 or 4 bits), the query's own token written on the way if it is
 // given; sequences of unequal length.
 //
-// The rows that the sequences may see, in chunks of 128, form one flat list (sequence, kv head, chunk); every CTA, one per SM,
-// takes an equal contiguous range of it.  A producer warp streams the range through a ring of shared-memory stages, eight math
-// warps follow it, each with 16 rows of every chunk, and keep a running maximum, sum and output of their own, which are
-// joined when the CTA leaves a kv row.  A kv row that lies inside one range is finished there; of one that is cut each CTA
-// leaves a partial result (fp32), and kvm_window_join_kernel joins those in the order of the list.  Nothing is counted or
-// kept between calls.
+// The rows that the sequences may see, in chunks, form one flat list (sequence, kv head, chunk); every CTA takes an equal
+// contiguous range of it.  Its chunks stream through a ring of shared-memory stages; eight math warps, each with its own rows
+// of every chunk, keep a running maximum, sum and output of their own, which are joined when the CTA leaves a kv row.  A kv row
+// that lies inside one range is finished there; of one that is cut each CTA leaves a partial result (fp32), and
+// kvm_window_join_kernel joins those in the order of the list.  Nothing is counted or kept between calls.
 //
-// Bound by memory: a row is read once for all query heads of its kv head.  The products run on warp-level MMAs with the
-// cache rows on the M dimension and the query heads on N (8 or 16 columns).
+// A row is read once for all query heads of its kv head.  The products run on warp-level MMAs with the cache rows on the M
+// dimension and the query heads on N (8 or 16 columns).
 // 4 bits: the codes become f16 with one conversion instruction per two values.  q is scaled by a power of two per head into
 // f16's range.  A key group's scale multiplies the fp32 sum of its group; a value group's scale multiplies the weights, as
 // f16 relative to a running power of two R above all scales seen so far (the output is rescaled when R rises, as with the
@@ -25,31 +24,38 @@ namespace kvm {
 
 namespace {
 
-constexpr int kChunk = 128;                   // rows per chunk
 constexpr int kMathWarps = 8;
-constexpr int kTokThreads = (kMathWarps + 1) * 32;
 constexpr int kMaxStages = 8;
 constexpr int kBox = 16;                      // rows per TMA box (16 bits)
-constexpr int kMaxSmemBytes = 227 * 1024;
+constexpr int kSmemPerSm = 228 * 1024;        // of which every CTA takes 1 KB more than it asks for
 constexpr int kMaxBatch = 1024;               // sequences per launch
+constexpr float kLowest = -3e38f;             // running maximum before the first score
 
-template <int D, int BITS>
+// How a variant works.  4 bits: bound by the math warps (conversions and fixed latencies): two groups of 16 rows per warp
+// and chunk side by side, two CTAs per SM where the registers allow it, the copies (one per chunk) issued by math warp 0.
+// 16 bits: bound by memory: one CTA with deep stages and a producer warp of its own (many copies per chunk).
+template <int D, int BITS, int NH>
 struct TokGeom {
+  static constexpr int kTiles = BITS == 4 ? 2 : 1;               // groups of 16 rows per warp and chunk
+  static constexpr int kChunk = kMathWarps * 16 * kTiles;        // rows per chunk
+  static constexpr bool kProducer = BITS == 16;
+  static constexpr int kThreads = (kMathWarps + (kProducer ? 1 : 0)) * 32;
+  static constexpr int kCtas = BITS == 4 && NH == 1 ? 2 : 1;     // per SM
   static constexpr int kStageKv = BITS == 4 ? kChunk / 16 * Block4<D>::kBytes : 2 * kChunk * D * 2;
-  static constexpr int kBoxW = D >= 64 ? 64 : 32;   // elements per box
+  static constexpr int kBoxW = D >= 64 ? 64 : 32;                // elements per box
   static constexpr int kBlocks = D / kBoxW;
 };
 
 struct TokSmem {
-  int stage_bytes, q, ored, wred, bars, pre, total, stages;
-  __host__ __device__ TokSmem(int kv_bytes, int D, int G, int nb, int st) {
+  int stage_bytes, q, ored, vscale, wred, bars, pre, total;
+  __host__ __device__ TokSmem(int kv_bytes, int D, int G, int nb, int stages) {
     q = kv_bytes;                                            // [G][D] bf16 behind the stage's rows
     stage_bytes = (q + G * D * 2 + 1023) & ~1023;            // (boxes in the 128-byte swizzle start on 1024 bytes)
-    stages = st;
-    int off = st * stage_bytes;
+    int off = stages * stage_bytes;
     ored = off; off += kMathWarps * G * D * 4;
+    vscale = off; off += kMathWarps * 2 * 128;               // a warp's value scales as f16
     wred = off; off += 2 * kMathWarps * 16 * 4;
-    bars = off; off += 2 * kMaxStages * 8;
+    bars = off; off += 2 * kMaxStages * 8 + 16;              // full, empty, abort flag
     pre = off;  off += (2 * nb + 1) * 4;
     total = (off + 15) & ~15;
   }
@@ -63,6 +69,11 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -100,6 +111,12 @@ struct Seen {
     const int back = newest - (r - sp);
     return r < live && (r < sp ? r < sinks : (back < 0 ? back + ring : back) < limit);
   }
+  // rows [r, r + 16) (r a multiple of 16) as a bit mask; one lane per row where they are not plainly all seen
+  __device__ __forceinline__ unsigned group(int r, int lane) const {
+    const int first = r - sp, back = newest - first;  // of the first row
+    if (first >= 0 && r + 16 <= live && (limit == ring || (back >= 15 && back < limit))) return 0xffffu;
+    return __ballot_sync(0xffffffffu, visible(r + (lane & 15))) & 0xffffu;
+  }
 };
 
 // A place in the flat list.
@@ -120,14 +137,13 @@ struct Split {
   }
 };
 
-__device__ __forceinline__ int chunks_of(const WindowDev& W, int n) { return (W.live(n) + kChunk - 1) / kChunk; }
-
 // Tokens of every sequence (pre[nb + 1 ..]) and its chunks per kv row as a prefix (pre[0..nb]) in shared memory.
-__device__ __forceinline__ void build_prefix(const WindowDev& W, SeqInts lens, int extra, int b0, int nb, int* pre, int tid, int threads) {
+__device__ __forceinline__ void build_prefix(const WindowDev& W, SeqInts lens, int extra, int chunk, int b0, int nb, int* pre, int tid,
+                                             int threads) {
   for (int b = tid; b < nb; b += threads) {
     const int n = max(lens.at(b0 + b), -1) + extra;
     pre[nb + 1 + b] = n;
-    pre[b + 1] = chunks_of(W, n);
+    pre[b + 1] = (W.live(n) + chunk - 1) / chunk;
   }
   if (tid == 0) pre[0] = 0;
   __syncthreads();
@@ -149,7 +165,7 @@ __device__ __forceinline__ void build_prefix(const WindowDev& W, SeqInts lens, i
 }
 // sequence whose kv rows hold place f of the list
 __device__ __forceinline__ int find_seq(const int* pre, int nb, int Hkv, int f) {
-  int lo = 0, hi = nb - 1;  // last b with pre[b] * Hkv <= f among those that have chunks
+  int lo = 0, hi = nb - 1;  // last b with pre[b] * Hkv <= f: one that has chunks
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (pre[mid] * Hkv <= f) lo = mid; else hi = mid - 1;
@@ -157,26 +173,74 @@ __device__ __forceinline__ int find_seq(const int* pre, int nb, int Hkv, int f) 
   return lo;
 }
 
+// N 32-bit words from shared memory (16 N-byte, at most 16-byte, aligned)
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&x)[N], const void* p) {
+  if constexpr (N == 4) {
+    const uint4 y = *static_cast<const uint4*>(p);
+    x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+  } else if constexpr (N == 2) {
+    const uint2 y = *static_cast<const uint2*>(p);
+    x[0] = y.x; x[1] = y.y;
+  } else {
+    x[0] = *static_cast<const uint32_t*>(p);
+  }
+}
+
+// The new token's row into row rr of a 4-bit block, in the stage and in memory (whole warp; items of 4 channels of K, then V).
+template <int D>
+__device__ __forceinline__ void patch4(unsigned char* sb, unsigned char* gb, const bf16* kn, const bf16* vn, int rr, int lane) {
+  constexpr int NG = D / 32;
+#pragma unroll
+  for (int it = 0; it < (D == 128 ? 2 : 1); ++it) {
+    const int item = it * 32 + lane, value = item >= D / 4, c4 = value ? item - D / 4 : item;
+    const bool some = item < D / 2;
+    const uint2 x = some ? *reinterpret_cast<const uint2*>((value ? vn : kn) + c4 * 4) : make_uint2(0, 0);
+    unsigned am = __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu);
+    am = max(am & 0xffffu, am >> 16);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, d));  // 8 lanes hold a group
+    float inv;
+    const unsigned short sc = group_scale(am, inv);
+    const float2 f0 = unpack_bf16(x.x), f1 = unpack_bf16(x.y);
+    unsigned code = e2m1x2(level_of(f0.x, inv), level_of(f0.y, inv)) | e2m1x2(level_of(f1.x, inv), level_of(f1.y, inv)) << 8;
+    if (am >= 0x7f80u) code = 0;
+    const int grp = c4 >> 3, u = c4 & 7;
+    const int off = value ? Block4<D>::kValues + rr * (D / 2) + u * (2 * NG) + grp * 2
+                          : Block4<D>::kKeys + rr * (D / 2) + (u >> 1) * (4 * NG) + grp * 4 + (u & 1) * 2;
+    const int soff = value ? Block4<D>::kValueScales + (rr >> 1) * (4 * NG) + grp * 4 + (rr & 1) * 2
+                           : Block4<D>::kKeyScales + rr * (2 * NG) + grp * 2;
+    if (some) {
+      *reinterpret_cast<unsigned short*>(sb + off) = (unsigned short)code;
+      *reinterpret_cast<unsigned short*>(gb + off) = (unsigned short)code;
+      if (u == 0) {
+        *reinterpret_cast<unsigned short*>(sb + soff) = sc;
+        *reinterpret_cast<unsigned short*>(gb + soff) = sc;
+      }
+    }
+  }
+}
+
 }  // namespace
 
 template <int D, int BITS, int NH>
-__global__ void __launch_bounds__(kTokThreads, 1)
+__global__ void __launch_bounds__(TokGeom<D, BITS, NH>::kThreads, TokGeom<D, BITS, NH>::kCtas)
 kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, int b0, int nb, int stages,
                         int whole_rows, float scale_log2, float* __restrict__ partial, bf16* __restrict__ out, int* __restrict__ status,
                         const __grid_constant__ TokMaps maps) {
-  using GM = TokGeom<D, BITS>;
-  constexpr int NG = D / 32;       // groups of 32 channels
+  using GM = TokGeom<D, BITS, NH>;
+  constexpr int NG = D / 32, NT = GM::kTiles, CH = GM::kChunk;
+  constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(1024) unsigned char smem[];
   const TokSmem lay(GM::kStageKv, D, G, nb, stages);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + lay.bars);
   uint64_t* empty = full + kMaxStages;
   int* pre = reinterpret_cast<int*>(smem + lay.pre);
   const int* tokens = pre + nb + 1;
-  __shared__ int s_abort;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = reinterpret_cast<int*>(empty + kMaxStages);
+  const int tid = threadIdx.x, warp = __shfl_sync(kAll, tid >> 5, 0), lane = tid & 31;
   const int Hkv = W.Hkv, Hq = Hkv * G;
   const bool with_new = k_new.ptr != nullptr;
-  const int extra = with_new ? 1 : 0;  // lens are positions of the new tokens
 
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -184,14 +248,14 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
       tc::mbar_init(&empty[s], kMathWarps);
     }
     tc::fence_barrier_init();
-    s_abort = 0;
+    *abort_flag = 0;
   }
   pdl_trigger();  // (the join kernel may be staged; it waits for this grid)
   pdl_wait();
-  build_prefix(W, lens, extra, b0, nb, pre, tid, kTokThreads);
+  build_prefix(W, lens, with_new ? 1 : 0, CH, b0, nb, pre, tid, GM::kThreads);  // (with a new token lens are its positions)
   const int total_f = pre[nb] * Hkv;
 
-  // this CTA's range [f_begin, f_end)
+  // this CTA's range [f_begin, f_end) of the list
   int f_begin, f_end;
   if (whole_rows) {
     const Split sp(nb * Hkv, gridDim.x);
@@ -208,7 +272,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
   // sequences without tokens: zeros
   for (int b = blockIdx.x; b < nb; b += gridDim.x)
     if (pre[b + 1] == pre[b])
-      for (int i = tid; i < Hq * D / 8; i += kTokThreads)
+      for (int i = tid; i < Hq * D / 8; i += GM::kThreads)
         reinterpret_cast<uint4*>(out + (size_t)(b0 + b) * Hq * D)[i] = make_uint4(0, 0, 0, 0);
   if (nloc <= 0) return;
 
@@ -220,534 +284,489 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
     pl.h = rem / pl.n_chunks;
     pl.c = rem % pl.n_chunks;
   }
-  auto advance = [&](Place& p) {
-    if (++p.c < p.n_chunks) return;
+  auto next_row = [&](Place& p) {
     p.c = 0;
     if (++p.h < Hkv) return;
     p.h = 0;
     do { ++p.b; } while (p.b < nb && pre[p.b + 1] == pre[p.b]);
     if (p.b < nb) p.n_chunks = pre[p.b + 1] - pre[p.b];
   };
-  volatile int* abort_flag = &s_abort;
+  auto give_up = [&]() {
+    if (lane == 0) {
+      *abort_flag = 1;
+      atomicExch(status, KVM_ERR_DEVICE_TIMEOUT);
+    }
+  };
 
-  if (warp == kMathWarps) {
-    // ------------------------------------------------------------------------------------ producer
+  // Chunk `pp` of the list into stage s, by a whole warp.
+  Place pp = pl;
+  auto load = [&](int s, bool first_of_range) {
+    unsigned char* st = smem + s * lay.stage_bytes;
+    const int rows = min(CH, W.live(tokens[pp.b]) - pp.c * CH), groups = (rows + 15) >> 4;
+    const size_t kvrow = (size_t)(b0 + pp.b) * Hkv + pp.h;
+    const bool first = first_of_range || pp.c == 0;  // the kv row's queries come with its first chunk
+    if (lane == 0) {
+      const uint32_t bytes = (BITS == 4 ? (uint32_t)groups * Block4<D>::kBytes : (uint32_t)groups * (2u * 16u * D * 2u)) + (first ? (uint32_t)(G * D * 2) : 0u);
+      tc::mbar_arrive_expect_tx(&full[s], bytes);
+    }
+    __syncwarp();
+    if (BITS == 4) {
+      if (lane == 0)
+        tc::bulk_g2s(st, W.blocks + (kvrow * (W.rows / 16) + (size_t)pp.c * (CH / 16)) * Block4<D>::kBytes, groups * Block4<D>::kBytes, &full[s]);
+    } else {
+      const int y = (int)(kvrow * W.rows) + pp.c * CH;  // (all rows of a cache: below 2^31, checked on the host)
+      for (int j = lane; j < groups * GM::kBlocks * 2; j += 32) {
+        const int half = j / (groups * GM::kBlocks), k2 = j % (groups * GM::kBlocks), blk = k2 / groups, gr = k2 % groups;
+        tc::tma_load_2d(st + half * (CH * D * 2) + blk * (CH * GM::kBoxW * 2) + gr * (kBox * GM::kBoxW * 2), half ? &maps.v : &maps.k,
+                        blk * GM::kBoxW, y + gr * kBox, &full[s]);
+      }
+    }
+    if (first && lane < G) tc::bulk_g2s(st + lay.q + lane * D * 2, q.row(b0 + pp.b, pp.h * G + lane, 0), D * 2, &full[s]);
+    if (++pp.c == pp.n_chunks) next_row(pp);
+  };
+  if (GM::kProducer && warp == kMathWarps) {
+    int s = 0, parity = 0;
     for (int i = 0; i < nloc; ++i) {
-      const int s = i % stages;
       if (i >= stages) {
-        const bool ok = tc::mbar_wait(&empty[s], ((i / stages) - 1) & 1) && !*abort_flag;
-        if (!__all_sync(0xffffffffu, ok)) {
-          if (lane == 0) {
-            *abort_flag = 1;
-            atomicExch(status, KVM_ERR_DEVICE_TIMEOUT);
-            for (int j = i - stages; j < i; ++j) tc::mbar_wait_limit(&full[j % stages], (j / stages) & 1, 1 << 14);  // copies in flight
-          }
-          __syncwarp();
+        if (!__all_sync(kAll, tc::mbar_wait(&empty[s], parity ^ 1) && !*abort_flag)) {
+          give_up();
+          __nanosleep(1000000);  // copies in flight
           break;
         }
       }
-      unsigned char* st = smem + s * lay.stage_bytes;
-      const int n = tokens[pl.b];
-      const int rows = min(kChunk, W.live(n) - pl.c * kChunk), groups = (rows + 15) >> 4;
-      const size_t kvrow = (size_t)(b0 + pl.b) * Hkv + pl.h;
-      const bool first = i == 0 || pl.c == 0;
-      if (lane == 0) {
-        const uint32_t bytes = (BITS == 4 ? (uint32_t)groups * Block4<D>::kBytes : (uint32_t)groups * (2u * 16u * D * 2u)) + (first ? (uint32_t)(G * D * 2) : 0u);
-        tc::mbar_arrive_expect_tx(&full[s], bytes);
-      }
-      __syncwarp();
-      if (first && lane < G) tc::bulk_g2s(st + lay.q + lane * D * 2, q.row(b0 + pl.b, pl.h * G + lane, 0), D * 2, &full[s]);
-      if (BITS == 4) {
-        if (lane == 0)
-          tc::bulk_g2s(st, W.blocks + (kvrow * (W.rows / 16) + (size_t)pl.c * (kChunk / 16)) * Block4<D>::kBytes, groups * Block4<D>::kBytes, &full[s]);
-      } else {
-        const int y = (int)(kvrow * W.rows) + pl.c * kChunk;  // (all rows of a cache: below 2^31, checked on the host)
-        for (int j = lane; j < groups * GM::kBlocks * 2; j += 32) {
-          const int half = j / (groups * GM::kBlocks), k2 = j % (groups * GM::kBlocks), blk = k2 / groups, gr = k2 % groups;
-          tc::tma_load_2d(st + half * (kChunk * D * 2) + blk * (kChunk * GM::kBoxW * 2) + gr * (kBox * GM::kBoxW * 2), half ? &maps.v : &maps.k,
-                          blk * GM::kBoxW, y + gr * kBox, &full[s]);
-        }
-      }
-      advance(pl);
+      load(s, i == 0);
+      if (++s == stages) { s = 0; parity ^= 1; }
     }
     return;
   }
+  if (!GM::kProducer && warp == 0)
+    for (int i = 0; i < min(stages, nloc); ++i) load(i, i == 0);
 
-  // -------------------------------------------------------------------------------------- math warps
   const int g = lane >> 2, t = lane & 3;
   float* ored = reinterpret_cast<float*>(smem + lay.ored);          // [warp][G][D]
   float* wmax = reinterpret_cast<float*>(smem + lay.wred);          // [warp][16]
   float* wsum = wmax + kMathWarps * 16;
-  uint32_t qf[NH][D / 16][2];
-  float qs[NH][2];                 // softmax scale (log2) of this thread's heads 2t, 2t + 1
-  float o[NH][D / 16][4];          // output rows (channels) x heads
-  float m[NH][2], l[NH][2];
-  float r_ref = 0.f;               // 4 bits: the power of two that the weights are relative to (0: none yet)
-  unsigned r_bits = 0;             // its bf16 exponent field
-  const Place start = pl;
-  Seen seen(W, 0);
+  uint32_t* vsc = reinterpret_cast<uint32_t*>(smem + lay.vscale + warp * 256);
   bool ok = true;  // false: a wait ran out; the warp goes on without data so that it meets the others at their barriers
+  int s = 0, parity = 0;             // stage of the chunk, parity of its use
+  int rs = 0, rparity = 0;           // of the chunk before it
 
-  for (int i = 0; i < nloc; ++i) {
-    const int s = i % stages;
-    if (ok) {
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[s], (i / stages) & 1) && !*abort_flag);
-      if (!ok && lane == 0) {
-        *abort_flag = 1;
-        atomicExch(status, KVM_ERR_DEVICE_TIMEOUT);
-      }
+  for (int i = 0; i < nloc;) {  // kv rows, or what of them lies in the range
+    const int cnt = min(pl.n_chunks - pl.c, nloc - i), n = tokens[pl.b];
+    const Seen seen(W, n);
+    const int new_row = with_new ? W.row_of(n - 1) : -1;
+    uint32_t qf[NH][D / 16][2];      // queries as B fragments
+    float qs[NH][2];                 // softmax scale (log2) of this thread's heads 2t, 2t + 1
+    float o[NH][D / 16][4];          // output: channels x heads
+    float m[NH][2], l[NH][2];
+    unsigned r_bits = 0;             // 4 bits: R, as the exponent field of a bf16 pattern (0: none yet)
+#pragma unroll
+    for (int hb = 0; hb < NH; ++hb) {
+      m[hb][0] = m[hb][1] = kLowest;
+      l[hb][0] = l[hb][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) o[hb][j][0] = o[hb][j][1] = o[hb][j][2] = o[hb][j][3] = 0.f;
     }
-    unsigned char* st = smem + s * lay.stage_bytes;
-    const int n = tokens[pl.b];
-    if (i == 0 || pl.c == 0) {  // a new kv row: queries as B fragments
-      seen = Seen(W, n);
+
+    for (int j = 0; j < cnt; ++j) {
+      const int at = i + j;
+      // the stage of the chunk before this one, which the other warps are done with by now or soon, takes a further chunk
+      if (!GM::kProducer && warp == 0 && ok && at > 0 && at - 1 + stages < nloc) {
+        ok = __all_sync(kAll, tc::mbar_wait(&empty[rs], rparity) && !*abort_flag);
+        if (ok) load(rs, false);
+        else give_up();
+      }
+      if (ok) {
+        ok = __all_sync(kAll, tc::mbar_wait(&full[s], parity) && !*abort_flag);
+        if (!ok) give_up();
+      }
+      unsigned char* st = smem + s * lay.stage_bytes;
+      if (j == 0) {
 #pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-        const int head = hb * 8 + g;
-        const bf16* qrow = reinterpret_cast<const bf16*>(st + lay.q) + (size_t)min(head, G - 1) * D;
-        if (BITS == 4) {
-          uint4 x[NG];
-          unsigned amax = 0;
+        for (int hb = 0; hb < NH; ++hb) {
+          const bf16* qrow = reinterpret_cast<const bf16*>(st + lay.q) + (size_t)min(hb * 8 + g, G - 1) * D;
+          if (BITS == 4) {
+            uint32_t x[NG][4];
+            unsigned amax = 0;
 #pragma unroll
-          for (int n2 = 0; n2 < NG; ++n2) {
-            x[n2] = *reinterpret_cast<const uint4*>(qrow + n2 * 32 + t * 8);
-            const unsigned w[4] = {x[n2].x, x[n2].y, x[n2].z, x[n2].w};
+            for (int n2 = 0; n2 < NG; ++n2) {
+              lds(x[n2], qrow + n2 * 32 + t * 8);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) amax = __vmaxu2(amax, w[j] & 0x7fff7fffu);
-          }
-          amax = max(amax & 0xffffu, amax >> 16);
-          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          // largest magnitude into [2^14, 2^15): a value loses bits only if it is 2^28 below it.  (2^-e as a float: e in
-          // [-126, 127]; infinities and NaN stay what they are)
-          const int e = min(max((int)(amax >> 7) - 127, -112), 127);
-          const float up = __uint_as_float((unsigned)(127 + 14 - e) << 23 & 0x7f800000u);
-          const float upc = amax >= 0x7f80u ? 1.f : up;
-          float down = amax >= 0x7f80u ? 1.f : __uint_as_float((unsigned)max(127 - 14 + e, 1) << 23);
-#pragma unroll
-          for (int n2 = 0; n2 < NG; ++n2) {
-            const unsigned w[4] = {x[n2].x, x[n2].y, x[n2].z, x[n2].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack_bf16(w[j]);
-              qf[hb][n2 * 2 + (j >> 1)][j & 1] = pack_f16(f.x * upc, f.y * upc);
+              for (int e = 0; e < 4; ++e) amax = __vmaxu2(amax, x[n2][e] & 0x7fff7fffu);
             }
-          }
-          // this thread's scores are of heads 2t, 2t + 1: their factors lie in lanes 8t, 8t + 4
-          qs[hb][0] = __shfl_sync(0xffffffffu, down, 8 * t) * scale_log2;
-          qs[hb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4) * scale_log2;
-        } else {
+            amax = max(amax & 0xffffu, amax >> 16);
+            amax = max(amax, __shfl_xor_sync(kAll, amax, 1));
+            amax = max(amax, __shfl_xor_sync(kAll, amax, 2));
+            // largest magnitude into [2^14, 2^15): a value loses bits only if it is 2^28 below it (infinities and NaN stay
+            // what they are)
+            const int e = min(max((int)(amax >> 7) - 127, -112), 127);
+            const bool finite = amax < 0x7f80u;
+            const float up = finite ? __uint_as_float((unsigned)(127 + 14 - e) << 23) : 1.f;
+            const float down = finite ? __uint_as_float((unsigned)(127 - 14 + e) << 23) : 1.f;
 #pragma unroll
-          for (int blk = 0; blk < (D >= 64 ? D / 64 : 1); ++blk) {
+            for (int n2 = 0; n2 < NG; ++n2)
+#pragma unroll
+              for (int e2 = 0; e2 < 4; ++e2) {
+                const float2 f = unpack_bf16(x[n2][e2]);
+                qf[hb][n2 * 2 + (e2 >> 1)][e2 & 1] = pack_f16(f.x * up, f.y * up);
+              }
+            // this thread's scores are of heads 2t, 2t + 1: their factors lie in lanes 8t, 8t + 4
+            qs[hb][0] = __shfl_sync(kAll, down, 8 * t) * scale_log2;
+            qs[hb][1] = __shfl_sync(kAll, down, 8 * t + 4) * scale_log2;
+          } else {
             constexpr int PER = D >= 64 ? 4 : 2;  // k-steps per 64 (32) channels; a thread's channels are contiguous
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const uint2 x = *reinterpret_cast<const uint2*>(qrow + blk * 64 + t * (PER * 4) + j * 4);
-              qf[hb][blk * PER + j][0] = x.x;
-              qf[hb][blk * PER + j][1] = x.y;
-            }
+            for (int kk = 0; kk < D / 16; ++kk) lds(qf[hb][kk], qrow + (kk / PER) * 64 + t * (PER * 4) + (kk % PER) * 4);
+            qs[hb][0] = qs[hb][1] = scale_log2;
           }
-          qs[hb][0] = qs[hb][1] = scale_log2;
         }
-        m[hb][0] = m[hb][1] = -INFINITY;
-        l[hb][0] = l[hb][1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) o[hb][j][0] = o[hb][j][1] = o[hb][j][2] = o[hb][j][3] = 0.f;
       }
-      r_ref = 0.f;
-      r_bits = 0;
-    }
 
-    // ---- this warp's 16 rows
-    const int row0 = pl.c * kChunk + warp * 16;
-    const unsigned vis = __ballot_sync(0xffffffffu, seen.visible(row0 + (lane & 15))) & 0xffffu;
-    if (vis && ok) {
-      const size_t kvrow = (size_t)(b0 + pl.b) * Hkv + pl.h;
-      // the new token's row: into the stage (what was loaded there is stale) and into memory
+      // ---- this warp's rows: groups of 16, kMathWarps * 16 apart
+      const int row0 = (pl.c + j) * CH + warp * 16;
+      unsigned vis[NT], any = 0, all = 0xffffu;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        vis[u] = seen.group(row0 + u * (kMathWarps * 16), lane);
+        any |= vis[u];
+        all &= vis[u];
+      }
       bool patched = false;
-      if (with_new) {
-        const int nr = W.row_of(n - 1);
-        if ((nr >> 4) == (row0 >> 4)) {
-          patched = true;
-          const int rr = nr & 15;
-          const bf16* kn = k_new.row(b0 + pl.b, pl.h, 0);
-          const bf16* vn = v_new.row(b0 + pl.b, pl.h, 0);
-          if (BITS == 16) {
-            for (int j = lane; j < D / 4; j += 32) {  // 16-byte pieces of K, then of V
-              const bool value = j >= D / 8;
-              const int c = value ? j - D / 8 : j;
-              const uint4 x = *reinterpret_cast<const uint4*>((value ? vn : kn) + c * 8);
-              const int r = warp * 16 + rr;
-              unsigned char* base = st + (value ? kChunk * D * 2 : 0);
-              if (D >= 64) base += (c >> 3) * (kChunk * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-              else base += r * 64 + c * 16;
-              *reinterpret_cast<uint4*>(base) = x;
-              *reinterpret_cast<uint4*>((value ? W.v : W.k) + (kvrow * W.rows + nr) * D + c * 8) = x;
+      if (any && ok) {
+        // the new token's row: into the stage (what was loaded there is stale) and into memory
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const int r = row0 + u * (kMathWarps * 16);
+          if (with_new && (new_row >> 4) == (r >> 4)) {
+            patched = true;
+            const size_t kvrow = (size_t)(b0 + pl.b) * Hkv + pl.h;
+            const bf16* kn = k_new.row(b0 + pl.b, pl.h, 0);
+            const bf16* vn = v_new.row(b0 + pl.b, pl.h, 0);
+            if (BITS == 4) {
+              patch4<D>(st + (warp + u * kMathWarps) * Block4<D>::kBytes,
+                        W.blocks + (kvrow * (W.rows / 16) + (new_row >> 4)) * Block4<D>::kBytes, kn, vn, new_row & 15, lane);
+            } else {
+              for (int e = lane; e < D / 4; e += 32) {  // 16-byte pieces of K, then of V
+                const bool value = e >= D / 8;
+                const int c = value ? e - D / 8 : e, rr = new_row - (pl.c + j) * CH;
+                const uint4 x = *reinterpret_cast<const uint4*>((value ? vn : kn) + c * 8);
+                unsigned char* base = st + (value ? CH * D * 2 : 0);
+                if (D >= 64) base += (c >> 3) * (CH * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+                else base += rr * 64 + c * 16;
+                *reinterpret_cast<uint4*>(base) = x;
+                *reinterpret_cast<uint4*>((value ? W.v : W.k) + (kvrow * W.rows + new_row) * D + c * 8) = x;
+              }
             }
-          } else {
-            unsigned char* sb = st + warp * Block4<D>::kBytes;
-            unsigned char* gb = W.blocks + (kvrow * (W.rows / 16) + (nr >> 4)) * Block4<D>::kBytes;
+            __syncwarp();
+          }
+        }
+        if (BITS == 4 && all != 0xffffu) {  // rows that are not to be seen: scale 0 and code 0, they add nothing
+          patched = true;
 #pragma unroll
-            for (int it = 0; it < (D == 128 ? 2 : 1); ++it) {  // items: 4 channels of K, then of V
-              const int item = it * 32 + lane, value = item >= D / 4, c4 = value ? item - D / 4 : item;
-              const bool live_item = item < D / 2;
-              const uint2 x = live_item ? *reinterpret_cast<const uint2*>((value ? vn : kn) + c4 * 4) : make_uint2(0, 0);
-              unsigned am = __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu);
-              am = max(am & 0xffffu, am >> 16);
-#pragma unroll
-              for (int d2 = 1; d2 < 8; d2 <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, d2));
-              float inv;
-              const unsigned short sc = group_scale(am, inv);
-              const float2 f0 = unpack_bf16(x.x), f1 = unpack_bf16(x.y);
-              unsigned code = e2m1x2(level_of(f0.x, inv), level_of(f0.y, inv)) | e2m1x2(level_of(f1.x, inv), level_of(f1.y, inv)) << 8;
-              if (am >= 0x7f80u) code = 0;
-              const int grp = c4 >> 3, u = c4 & 7;
-              const int off = value ? Block4<D>::kValues + rr * (D / 2) + u * (2 * NG) + grp * 2
-                                    : Block4<D>::kKeys + rr * (D / 2) + (u >> 1) * (4 * NG) + grp * 4 + (u & 1) * 2;
-              const int soff = value ? Block4<D>::kValueScales + (rr >> 1) * (4 * NG) + grp * 4 + (rr & 1) * 2
-                                     : Block4<D>::kKeyScales + rr * (2 * NG) + grp * 2;
-              if (live_item) {
-                *reinterpret_cast<unsigned short*>(sb + off) = (unsigned short)code;
-                *reinterpret_cast<unsigned short*>(gb + off) = (unsigned short)code;
-                if (u == 0) {
-                  *reinterpret_cast<unsigned short*>(sb + soff) = sc;
-                  *reinterpret_cast<unsigned short*>(gb + soff) = sc;
-                }
+          for (int u = 0; u < NT; ++u) {
+            unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
+            for (int e = lane; e < 16 * NG; e += 32) {
+              const int rr = e / NG, grp = e % NG;
+              if (!((vis[u] >> rr) & 1)) {
+                *reinterpret_cast<unsigned short*>(sb + Block4<D>::kKeyScales + rr * (2 * NG) + grp * 2) = 0;
+                *reinterpret_cast<unsigned short*>(sb + Block4<D>::kValueScales + (rr >> 1) * (4 * NG) + grp * 4 + (rr & 1) * 2) = 0;
               }
             }
           }
           __syncwarp();
         }
-      }
-      if (BITS == 4 && vis != 0xffffu) {  // rows that are not to be seen: scale 0 (whatever they hold, they add nothing)
-        patched = true;
-        unsigned char* sb = st + warp * Block4<D>::kBytes;
-        for (int j = lane; j < 16 * NG; j += 32) {
-          const int rr = j / NG, grp = j % NG;
-          if (!((vis >> rr) & 1)) {
-            *reinterpret_cast<unsigned short*>(sb + Block4<D>::kKeyScales + rr * (2 * NG) + grp * 2) = 0;
-            *reinterpret_cast<unsigned short*>(sb + Block4<D>::kValueScales + (rr >> 1) * (4 * NG) + grp * 4 + (rr & 1) * 2) = 0;
-          }
-        }
-        __syncwarp();
-      }
 
-      // ---- scores: rows g, g + 8 x heads 2t, 2t + 1
-      float sc[NH][4];
+        bool raise = false;
+        float r_alpha = 1.f;
+        if (BITS == 4) {  // the value scales relative to R as f16, each lane a pair of rows' of a group
+          uint32_t x[NT];
+          unsigned top = 0;
 #pragma unroll
-      for (int hb = 0; hb < NH; ++hb) sc[hb][0] = sc[hb][1] = sc[hb][2] = sc[hb][3] = 0.f;
-      if (BITS == 4) {
-        const unsigned char* sb = st + warp * Block4<D>::kBytes;
-        uint32_t kw[2][NG];
-        float ks[2][NG];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int rr = g + 8 * r;
-          const unsigned char* p = sb + Block4<D>::kKeys + rr * (D / 2) + t * (4 * NG);
-          const unsigned char* sp = sb + Block4<D>::kKeyScales + rr * (2 * NG);
-          if (NG == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(p);
-            kw[r][0] = x.x; kw[r][NG > 1 ? 1 : 0] = x.y; kw[r][NG > 2 ? 2 : 0] = x.z; kw[r][NG > 3 ? 3 : 0] = x.w;
-            const uint2 y = *reinterpret_cast<const uint2*>(sp);
-            ks[r][0] = __uint_as_float(y.x << 16); ks[r][NG > 1 ? 1 : 0] = __uint_as_float(y.x & 0xffff0000u);
-            ks[r][NG > 2 ? 2 : 0] = __uint_as_float(y.y << 16); ks[r][NG > 3 ? 3 : 0] = __uint_as_float(y.y & 0xffff0000u);
-          } else if (NG == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            kw[r][0] = x.x; kw[r][NG > 1 ? 1 : 0] = x.y;
-            const unsigned y = *reinterpret_cast<const unsigned*>(sp);
-            ks[r][0] = __uint_as_float(y << 16); ks[r][NG > 1 ? 1 : 0] = __uint_as_float(y & 0xffff0000u);
-          } else {
-            kw[r][0] = *reinterpret_cast<const unsigned*>(p);
-            ks[r][0] = __uint_as_float((unsigned)*reinterpret_cast<const unsigned short*>(sp) << 16);
+          for (int u = 0; u < NT; ++u) {
+            x[u] = lane < 8 * NG ? *reinterpret_cast<const uint32_t*>(st + (warp + u * kMathWarps) * Block4<D>::kBytes + Block4<D>::kValueScales + lane * 4) : 0u;
+            // the exponent of the largest of them (NaN does not count: it reaches its own group only)
+            const unsigned x0 = x[u] & 0xffffu, x1 = x[u] >> 16;
+            top = max(top, max(x0 < 0x7f80u ? x0 : 0u, x1 < 0x7f80u ? x1 : 0u));
           }
-        }
-#pragma unroll
-        for (int n2 = 0; n2 < NG; ++n2) {
-          uint32_t a[4], c[4];
-          e2m1_to_f16x2(kw[0][n2], a[0], a[1], a[2], a[3]);
-          e2m1_to_f16x2(kw[1][n2], c[0], c[1], c[2], c[3]);
-#pragma unroll
-          for (int hb = 0; hb < NH; ++hb) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(acc, a[0], c[0], a[1], c[1], qf[hb][n2 * 2][0], qf[hb][n2 * 2][1]);
-            mma_f16(acc, a[2], c[2], a[3], c[3], qf[hb][n2 * 2 + 1][0], qf[hb][n2 * 2 + 1][1]);
-            sc[hb][0] = fmaf(ks[0][n2], acc[0], sc[hb][0]);
-            sc[hb][1] = fmaf(ks[0][n2], acc[1], sc[hb][1]);
-            sc[hb][2] = fmaf(ks[1][n2], acc[2], sc[hb][2]);
-            sc[hb][3] = fmaf(ks[1][n2], acc[3], sc[hb][3]);
-          }
-        }
-      } else {
-        const int r = warp * 16 + g;
-#pragma unroll
-        for (int blk = 0; blk < GM::kBlocks; ++blk) {
-          constexpr int PIECES = GM::kBoxW / 32;  // 16-byte pieces per thread and row: 2 (64 channels) or 1
-#pragma unroll
-          for (int j = 0; j < PIECES; ++j) {
-            const int c = t * PIECES + j;
-            uint4 x, y;
-            if (D >= 64) {
-              const unsigned char* base = st + blk * (kChunk * 128) + r * 128 + ((c ^ (r & 7)) << 4);
-              x = *reinterpret_cast<const uint4*>(base);
-              y = *reinterpret_cast<const uint4*>(base + 8 * 128);
-            } else {
-              const unsigned char* base = st + r * 64 + c * 16;
-              x = *reinterpret_cast<const uint4*>(base);
-              y = *reinterpret_cast<const uint4*>(base + 8 * 64);
-            }
-#pragma unroll
-            for (int hb = 0; hb < NH; ++hb) {
-              const int kk = (blk * PIECES + j) * 2;
-              mma_bf16(sc[hb], x.x, y.x, x.y, y.y, qf[hb][kk][0], qf[hb][kk][1]);
-              mma_bf16(sc[hb], x.z, y.z, x.w, y.w, qf[hb][kk + 1][0], qf[hb][kk + 1][1]);
-            }
-          }
-        }
-      }
-      const bool see0 = (vis >> g) & 1, see1 = (vis >> (g + 8)) & 1;
-
-      // ---- running maximum (raised when a tile exceeds it by 2^8), weights
-      float alpha[NH][2];
-      bool raise = false;
-#pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[hb][j] = ((j < 2) ? see0 : see1) ? sc[hb][j] * qs[hb][j & 1] : -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float x = fmaxf(sc[hb][j], sc[hb][j + 2]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const bool up = x > m[hb][j] + 8.f || (m[hb][j] == -INFINITY && x > -INFINITY);
-          alpha[hb][j] = 1.f;
-          if (up) {
-            alpha[hb][j] = m[hb][j] == -INFINITY ? 0.f : ex2(m[hb][j] - x);
-            m[hb][j] = x;
+          top = __reduce_max_sync(kAll, top) & 0x7f80u;
+          if (top > r_bits + (6u << 7) || (r_bits == 0 && top)) {  // a scale is below 2^7 R, a weight at most 2^8: f16 holds the product
+            r_alpha = r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
+            r_bits = top;
             raise = true;
           }
+          const float inv = __uint_as_float((254u - (r_bits >> 7)) << 23);
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+            if (lane < 8 * NG) vsc[u * 32 + lane] = pack_f16(__uint_as_float(x[u] << 16) * inv, __uint_as_float(x[u] & 0xffff0000u) * inv);
+          __syncwarp();
         }
-      }
-      float r_alpha = 1.f;
-      if (BITS == 4) {
-        // the exponent of the largest value scale of these rows (NaN does not count: it reaches its own group only)
-        const unsigned char* sb = st + warp * Block4<D>::kBytes + Block4<D>::kValueScales;
-        unsigned x = lane < 8 * NG ? *reinterpret_cast<const unsigned*>(sb + lane * 4) : 0u;
-        const unsigned x0 = x & 0xffffu, x1 = x >> 16;
-        x = max(x0 < 0x7f80u ? x0 : 0u, x1 < 0x7f80u ? x1 : 0u);
-        x = __reduce_max_sync(0xffffffffu, x) & 0x7f80u;
-        if (x > r_bits + (6u << 7) || (r_bits == 0 && x)) {  // a scale is below 2^7 R, a weight at most 2^8: f16 holds the product
-          const unsigned old = r_bits;
-          r_bits = x;
-          r_alpha = old ? __uint_as_float((unsigned)max(127 + (int)(old >> 7) - (int)(x >> 7), 0) << 23) : 0.f;
-          r_ref = __uint_as_float(x << 16);
-          raise = true;
+
+        // ---- scores: rows g, g + 8 x heads 2t, 2t + 1
+        float sc[NT][NH][4];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+#pragma unroll
+          for (int hb = 0; hb < NH; ++hb) sc[u][hb][0] = sc[u][hb][1] = sc[u][hb][2] = sc[u][hb][3] = 0.f;
+          if constexpr (BITS == 4) {
+            const unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
+            uint32_t kw[2][NG];
+            float ks[2][NG];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int rr = g + 8 * r;
+              lds(kw[r], sb + Block4<D>::kKeys + rr * (D / 2) + t * (4 * NG));
+              const unsigned char* sp = sb + Block4<D>::kKeyScales + rr * (2 * NG);
+              if constexpr (NG == 1) {
+                ks[r][0] = __uint_as_float((unsigned)*reinterpret_cast<const unsigned short*>(sp) << 16);
+              } else {
+                uint32_t y[NG / 2];
+                lds(y, sp);
+#pragma unroll
+                for (int e = 0; e < NG; ++e) ks[r][e] = __uint_as_float((e & 1) ? y[e / 2] & 0xffff0000u : y[e / 2] << 16);
+              }
+            }
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) {
+              uint32_t a[4], c[4];
+              e2m1_to_f16x2(kw[0][n2], a[0], a[1], a[2], a[3]);
+              e2m1_to_f16x2(kw[1][n2], c[0], c[1], c[2], c[3]);
+#pragma unroll
+              for (int hb = 0; hb < NH; ++hb) {
+                float acc[4];
+                mma_f16_zero(acc, a[0], c[0], a[1], c[1], qf[hb][n2 * 2][0], qf[hb][n2 * 2][1]);
+                mma_f16(acc, a[2], c[2], a[3], c[3], qf[hb][n2 * 2 + 1][0], qf[hb][n2 * 2 + 1][1]);
+                sc[u][hb][0] = fmaf(ks[0][n2], acc[0], sc[u][hb][0]);
+                sc[u][hb][1] = fmaf(ks[0][n2], acc[1], sc[u][hb][1]);
+                sc[u][hb][2] = fmaf(ks[1][n2], acc[2], sc[u][hb][2]);
+                sc[u][hb][3] = fmaf(ks[1][n2], acc[3], sc[u][hb][3]);
+              }
+            }
+          } else {
+            const int r = warp * 16 + g;
+#pragma unroll
+            for (int blk = 0; blk < GM::kBlocks; ++blk) {
+              constexpr int PIECES = GM::kBoxW / 32;  // 16-byte pieces per thread and row: 2 (64 channels) or 1
+#pragma unroll
+              for (int pc = 0; pc < PIECES; ++pc) {
+                const int c = t * PIECES + pc;
+                const unsigned char* base = D >= 64 ? st + blk * (CH * 128) + r * 128 + ((c ^ (r & 7)) << 4) : st + r * 64 + c * 16;
+                uint32_t x[4], y[4];
+                lds(x, base);
+                lds(y, base + 8 * (D >= 64 ? 128 : 64));
+#pragma unroll
+                for (int hb = 0; hb < NH; ++hb) {
+                  const int kk = (blk * PIECES + pc) * 2;
+                  mma_bf16(sc[u][hb], x[0], y[0], x[1], y[1], qf[hb][kk][0], qf[hb][kk][1]);
+                  mma_bf16(sc[u][hb], x[2], y[2], x[3], y[3], qf[hb][kk + 1][0], qf[hb][kk + 1][1]);
+                }
+              }
+            }
+          }
         }
-      }
-      if (__any_sync(0xffffffffu, raise)) {
+
+        // ---- running maximum (raised when a chunk exceeds it by 2^8), weights
+        float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
-          l[hb][0] *= alpha[hb][0];
-          l[hb][1] *= alpha[hb][1];
-          const float a0 = alpha[hb][0] * r_alpha, a1 = alpha[hb][1] * r_alpha;
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            o[hb][j][0] *= a0;
-            o[hb][j][1] *= a1;
-            o[hb][j][2] *= a0;
-            o[hb][j][3] *= a1;
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[u][hb][e] *= qs[hb][e & 1];
+          if (all != 0xffffu) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!((vis[u] >> (g + (e >> 1) * 8)) & 1)) sc[u][hb][e] = -INFINITY;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(sc[0][hb][e], sc[0][hb][e + 2]);
+            if (NT == 2) x = fmaxf(x, fmaxf(sc[NT - 1][hb][e], sc[NT - 1][hb][e + 2]));
+            x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(kAll, x, 16));
+            const bool up = x > m[hb][e] + 8.f;
+            alpha[hb][e] = up ? ex2(m[hb][e] - x) : 1.f;
+            m[hb][e] = up ? x : m[hb][e];
+            raise |= up;
           }
         }
-      }
-      uint32_t pb[NH][2];  // weights as B fragments: rows (2t, 2t + 1), (2t + 8, 2t + 9) of head g
+        if (__any_sync(kAll, raise)) {
 #pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-        float p[4];
+          for (int hb = 0; hb < NH; ++hb) {
+            l[hb][0] *= alpha[hb][0];
+            l[hb][1] *= alpha[hb][1];
+            const float a0 = alpha[hb][0] * r_alpha, a1 = alpha[hb][1] * r_alpha;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float mm = m[hb][j & 1] == -INFINITY ? 0.f : m[hb][j & 1];
-          p[j] = ex2(sc[hb][j] - mm);
-        }
-        l[hb][0] += p[0] + p[2];
-        l[hb][1] += p[1] + p[3];
-        pb[hb][0] = movmatrix_trans(BITS == 4 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));
-        pb[hb][1] = movmatrix_trans(BITS == 4 ? pack_f16(p[2], p[3]) : pack_bf16(p[2], p[3]));
-      }
-
-      // ---- output += V^T P
-      if (BITS == 4) {
-        const unsigned char* sb = st + warp * Block4<D>::kBytes;
-        // value scales of row pairs t and t + 4, relative to R, as f16x2
-        const float inv = __uint_as_float((254u - (r_bits >> 7)) << 23);
-        uint32_t vs[2][NG];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const unsigned char* p = sb + Block4<D>::kValueScales + (t + 4 * r) * (4 * NG);
-          uint32_t x[4] = {0, 0, 0, 0};
-          if (NG == 4) {
-            const uint4 y = *reinterpret_cast<const uint4*>(p);
-            x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-          } else if (NG == 2) {
-            const uint2 y = *reinterpret_cast<const uint2*>(p);
-            x[0] = y.x; x[1] = y.y;
-          } else {
-            x[0] = *reinterpret_cast<const uint32_t*>(p);
-          }
-#pragma unroll
-          for (int n2 = 0; n2 < NG; ++n2) {
-            vs[r][n2] = pack_f16(__uint_as_float(x[n2] << 16) * inv, __uint_as_float(x[n2] & 0xffff0000u) * inv);
-          }
-        }
-        constexpr int NWD = NG > 1 ? NG / 2 : 1;  // 32-bit words of codes per thread and row
-        uint32_t vw[4][NWD];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int rr = 2 * t + (r & 1) + 8 * (r >> 1);
-          const unsigned char* p = sb + Block4<D>::kValues + rr * (D / 2) + g * (2 * NG);
-          if (NG == 4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            vw[r][0] = x.x; vw[r][NWD - 1] = x.y;
-          } else if (NG == 2) {
-            vw[r][0] = *reinterpret_cast<const unsigned*>(p);
-          } else {
-            vw[r][0] = *reinterpret_cast<const unsigned short*>(p);
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < NWD; ++w) {
-          // rows (2t, 2t + 1) and (2t + 8, 2t + 9) side by side in a byte: even channels in e, odd ones in d
-          uint32_t e[2], d[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            e[r] = (vw[2 * r][w] & 0x0f0f0f0fu) | ((vw[2 * r + 1][w] << 4) & 0xf0f0f0f0u);
-            d[r] = ((vw[2 * r][w] >> 4) & 0x0f0f0f0fu) | (vw[2 * r + 1][w] & 0xf0f0f0f0u);
-          }
-          uint32_t ea[4], da[4], eb[4], db[4];
-          e2m1_to_f16x2(e[0], ea[0], ea[1], ea[2], ea[3]);
-          e2m1_to_f16x2(d[0], da[0], da[1], da[2], da[3]);
-          e2m1_to_f16x2(e[1], eb[0], eb[1], eb[2], eb[3]);
-          e2m1_to_f16x2(d[1], db[0], db[1], db[2], db[3]);
-#pragma unroll
-          for (int half = 0; half < (NG > 1 ? 2 : 1); ++half) {
-            const int n2 = w * 2 + half;
-#pragma unroll
-            for (int hb = 0; hb < NH; ++hb) {
-              const uint32_t p0 = mul_f16x2(pb[hb][0], vs[0][n2]), p1 = mul_f16x2(pb[hb][1], vs[1][n2]);
-#pragma unroll
-              for (int j = 0; j < 2; ++j)  // channels 32 n2 + 4 g + 2 j (rows g) and + 1 (rows g + 8)
-                mma_f16(o[hb][n2 * 2 + j], ea[half * 2 + j], da[half * 2 + j], eb[half * 2 + j], db[half * 2 + j], p0, p1);
+            for (int e = 0; e < D / 16; ++e) {
+              o[hb][e][0] *= a0;
+              o[hb][e][1] *= a1;
+              o[hb][e][2] *= a0;
+              o[hb][e][3] *= a1;
             }
           }
         }
+        uint32_t pb[NT][NH][2];  // weights as B fragments: rows (2t, 2t + 1), (2t + 8, 2t + 9) of head g
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int hb = 0; hb < NH; ++hb) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = ex2(sc[u][hb][e] - m[hb][e & 1]);
+            l[hb][0] += p[0] + p[2];
+            l[hb][1] += p[1] + p[3];
+            pb[u][hb][0] = movmatrix_trans(BITS == 4 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));
+            pb[u][hb][1] = movmatrix_trans(BITS == 4 ? pack_f16(p[2], p[3]) : pack_bf16(p[2], p[3]));
+          }
+
+        // ---- output += V^T P
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          if constexpr (BITS == 4) {
+            const unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
+            uint32_t vs[2][NG];  // value scales of row pairs t and t + 4
+            lds(vs[0], vsc + u * 32 + t * NG);
+            lds(vs[1], vsc + u * 32 + (t + 4) * NG);
+            constexpr int NWD = NG > 1 ? NG / 2 : 1;  // 32-bit words of codes per thread and row
+            uint32_t vw[4][NWD];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const unsigned char* p = sb + Block4<D>::kValues + (2 * t + (r & 1) + 8 * (r >> 1)) * (D / 2) + g * (2 * NG);
+              if constexpr (NG > 1) lds(vw[r], p);
+              else vw[r][0] = *reinterpret_cast<const unsigned short*>(p);
+            }
+#pragma unroll
+            for (int w = 0; w < NWD; ++w) {
+              // rows (2t, 2t + 1) and (2t + 8, 2t + 9) side by side in a byte: even channels in e, odd ones in d
+              uint32_t e[2], d[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                e[r] = (vw[2 * r][w] & 0x0f0f0f0fu) | ((vw[2 * r + 1][w] << 4) & 0xf0f0f0f0u);
+                d[r] = ((vw[2 * r][w] >> 4) & 0x0f0f0f0fu) | (vw[2 * r + 1][w] & 0xf0f0f0f0u);
+              }
+              uint32_t ea[4], da[4], eb[4], db[4];
+              e2m1_to_f16x2(e[0], ea[0], ea[1], ea[2], ea[3]);
+              e2m1_to_f16x2(d[0], da[0], da[1], da[2], da[3]);
+              e2m1_to_f16x2(e[1], eb[0], eb[1], eb[2], eb[3]);
+              e2m1_to_f16x2(d[1], db[0], db[1], db[2], db[3]);
+#pragma unroll
+              for (int half = 0; half < (NG > 1 ? 2 : 1); ++half) {
+                const int n2 = w * 2 + half;
+#pragma unroll
+                for (int hb = 0; hb < NH; ++hb) {
+                  const uint32_t p0 = mul_f16x2(pb[u][hb][0], vs[0][n2]), p1 = mul_f16x2(pb[u][hb][1], vs[1][n2]);
+#pragma unroll
+                  for (int y = 0; y < 2; ++y)  // channels 32 n2 + 4 g + 2 y (rows g) and + 1 (rows g + 8)
+                    mma_f16(o[hb][n2 * 2 + y], ea[half * 2 + y], da[half * 2 + y], eb[half * 2 + y], db[half * 2 + y], p0, p1);
+                }
+              }
+            }
+          } else {
+            const unsigned char* vb = st + CH * D * 2;
+#pragma unroll
+            for (int blk = 0; blk < GM::kBlocks; ++blk) {
+              constexpr int WORDS = D >= 64 ? 4 : 2;
+              uint32_t x[4][WORDS];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int rr = warp * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
+                lds(x[r], D >= 64 ? vb + blk * (CH * 128) + rr * 128 + ((g ^ (rr & 7)) << 4) : vb + rr * 64 + g * 8);
+                if (all != 0xffffu && !((vis[u] >> (rr & 15)) & 1)) {  // (0 x NaN)
+#pragma unroll
+                  for (int w = 0; w < WORDS; ++w) x[r][w] = 0;
+                }
+              }
+#pragma unroll
+              for (int w = 0; w < WORDS; ++w) {
+                const uint32_t a0 = __byte_perm(x[0][w], x[1][w], 0x5410), a1 = __byte_perm(x[0][w], x[1][w], 0x7632);
+                const uint32_t a2 = __byte_perm(x[2][w], x[3][w], 0x5410), a3 = __byte_perm(x[2][w], x[3][w], 0x7632);
+#pragma unroll
+                for (int hb = 0; hb < NH; ++hb) mma_bf16(o[hb][blk * 4 + w], a0, a1, a2, a3, pb[u][hb][0], pb[u][hb][1]);
+              }
+            }
+          }
+        }
+        if (patched) tc::fence_proxy_async();  // before the next copy into this stage
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[s]);
+      rs = s;
+      rparity = parity;
+      if (++s == stages) { s = 0; parity ^= 1; }
+    }
+
+    // ---- join the warps
+#pragma unroll
+    for (int hb = 0; hb < NH; ++hb) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[hb][e];
+        x += __shfl_xor_sync(kAll, x, 4);
+        x += __shfl_xor_sync(kAll, x, 8);
+        x += __shfl_xor_sync(kAll, x, 16);
+        const int head = hb * 8 + 2 * t + e;
+        if (g == 0) {
+          wmax[warp * 16 + head] = m[hb][e];
+          wsum[warp * 16 + head] = x;
+        }
+        if (head < G) {
+          float* dst = ored + ((size_t)warp * G + head) * D;
+          const float up = BITS == 4 ? __uint_as_float(r_bits << 16) : 1.f;
+#pragma unroll
+          for (int k2 = 0; k2 < D / 16; ++k2) {
+            // 4 bits: channels 32 (k2/2) + 4 g + 2 (k2%2) + {0, 1};  16 bits: 64 (k2/4) + 8 g + 2 (k2%4) + {0, 1}, and for
+            // D = 32: 4 g + 2 k2 + {0, 1}
+            const int ch = BITS == 4 || D == 32 ? (k2 >> 1) * 32 + 4 * g + 2 * (k2 & 1) : (k2 >> 2) * 64 + 8 * g + 2 * (k2 & 3);
+            *reinterpret_cast<float2*>(dst + ch) = make_float2(o[hb][k2][e] * up, o[hb][k2][e + 2] * up);
+          }
+        }
+      }
+    }
+    math_sync();
+    const bool whole = pl.c == 0 && cnt == pl.n_chunks;
+    const int slot = pl.c > 0 ? 0 : 1;  // of a cut row's partial results: it goes on here, or it begins here
+    for (int x = tid; x < G * D / 2; x += kMathWarps * 32) {
+      const int head = x / (D / 2), ch = (x % (D / 2)) * 2;
+      float mx = kLowest;
+#pragma unroll
+      for (int w = 0; w < kMathWarps; ++w) mx = fmaxf(mx, wmax[w * 16 + head]);
+      float sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMathWarps; ++w) {
+        const float f = ex2(wmax[w * 16 + head] - mx);
+        const float2 y = *reinterpret_cast<const float2*>(ored + ((size_t)w * G + head) * D + ch);
+        sum = fmaf(wsum[w * 16 + head], f, sum);
+        a0 = fmaf(y.x, f, a0);
+        a1 = fmaf(y.y, f, a1);
+      }
+      if (whole) {
+        *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + pl.b) * Hq + pl.h * G + head) * D + ch) = pack_bf16(a0 / sum, a1 / sum);
       } else {
-        const unsigned char* vb = st + kChunk * D * 2;
-#pragma unroll
-        for (int blk = 0; blk < GM::kBlocks; ++blk) {
-          uint4 x[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int rr = warp * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
-            if (D >= 64) {
-              x[r] = *reinterpret_cast<const uint4*>(vb + blk * (kChunk * 128) + rr * 128 + ((g ^ (rr & 7)) << 4));
-            } else {
-              const uint2 y = *reinterpret_cast<const uint2*>(vb + rr * 64 + g * 8);
-              x[r] = make_uint4(y.x, y.y, 0, 0);
-            }
-            if (vis != 0xffffu && !((vis >> (rr & 15)) & 1)) x[r] = make_uint4(0, 0, 0, 0);  // (0 x NaN)
-          }
-          const uint32_t* a = &x[0].x;
-          const uint32_t* b = &x[1].x;
-          const uint32_t* c = &x[2].x;
-          const uint32_t* d = &x[3].x;
-          constexpr int WORDS = D >= 64 ? 4 : 2;
-#pragma unroll
-          for (int w = 0; w < WORDS; ++w) {
-            const uint32_t a0 = __byte_perm(a[w], b[w], 0x5410), a1 = __byte_perm(a[w], b[w], 0x7632);
-            const uint32_t a2 = __byte_perm(c[w], d[w], 0x5410), a3 = __byte_perm(c[w], d[w], 0x7632);
-#pragma unroll
-            for (int hb = 0; hb < NH; ++hb) mma_bf16(o[hb][blk * 4 + w], a0, a1, a2, a3, pb[hb][0], pb[hb][1]);
-          }
-        }
+        float* dst = partial + ((size_t)blockIdx.x * 2 + slot) * partial_floats(D, G) + (size_t)head * (D + 2);
+        *reinterpret_cast<float2*>(dst + 2 + ch) = make_float2(a0, a1);
+        if (ch == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, sum);
       }
-      if (patched) tc::fence_proxy_async();  // before the next copy into this stage
     }
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&empty[s]);
-
-    // ---- the last chunk of a kv row, or of the range: join the warps
-    const Place here = pl;
-    const bool row_ends = here.c == here.n_chunks - 1;
-    advance(pl);
-    if (row_ends || i == nloc - 1) {
-#pragma unroll
-      for (int hb = 0; hb < NH; ++hb) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float x = l[hb][j];
-          x += __shfl_xor_sync(0xffffffffu, x, 4);
-          x += __shfl_xor_sync(0xffffffffu, x, 8);
-          x += __shfl_xor_sync(0xffffffffu, x, 16);
-          if (g == 0) {
-            wmax[warp * 16 + hb * 8 + 2 * t + j] = m[hb][j];
-            wsum[warp * 16 + hb * 8 + 2 * t + j] = x;
-          }
-          const int head = hb * 8 + 2 * t + j;
-          if (head < G) {
-            float* dst = ored + ((size_t)warp * G + head) * D;
-            const float up = BITS == 4 ? r_ref : 1.f;
-#pragma unroll
-            for (int k2 = 0; k2 < D / 16; ++k2) {
-              // 4 bits: channels 32 (k2/2) + 4 g + 2 (k2%2) + {0, 1};  16 bits: 64 (k2/4) + 8 g + 2 (k2%4) + {0, 1}, and for
-              // D = 32: 4 g + 2 k2 + {0, 1}
-              const int ch = BITS == 4 || D == 32 ? (k2 >> 1) * 32 + 4 * g + 2 * (k2 & 1) : (k2 >> 2) * 64 + 8 * g + 2 * (k2 & 3);
-              *reinterpret_cast<float2*>(dst + ch) = make_float2(o[hb][k2][j] * up, o[hb][k2][j + 2] * up);
-            }
-          }
-        }
-      }
-      math_sync();
-      const int f_row = f_begin + i - here.c;  // place of the row's first chunk in the list
-      const bool whole = f_row >= f_begin && row_ends;
-      const int slot = here.b == start.b && here.h == start.h && start.c > 0 ? 0 : 1;  // goes on here, or begins here
-      for (int e = tid; e < G * D / 2; e += kMathWarps * 32) {
-        const int head = e / (D / 2), ch = (e % (D / 2)) * 2;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kMathWarps; ++w) mx = fmaxf(mx, wmax[w * 16 + head]);
-        const float mm = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll
-        for (int w = 0; w < kMathWarps; ++w) {
-          const float f = ex2(wmax[w * 16 + head] - mm);
-          const float2 x = *reinterpret_cast<const float2*>(ored + ((size_t)w * G + head) * D + ch);
-          sum = fmaf(wsum[w * 16 + head], f, sum);
-          a0 = fmaf(x.x, f, a0);
-          a1 = fmaf(x.y, f, a1);
-        }
-        if (whole) {
-          *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + here.b) * Hq + here.h * G + head) * D + ch) = pack_bf16(a0 / sum, a1 / sum);
-        } else {
-          float* dst = partial + ((size_t)blockIdx.x * 2 + slot) * partial_floats(D, G) + (size_t)head * (D + 2);
-          *reinterpret_cast<float2*>(dst + 2 + ch) = make_float2(a0, a1);
-          if (ch == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, sum);
-        }
-      }
-      math_sync();
-    }
+    math_sync();
+    i += cnt;
+    next_row(pl);
   }
+  if (!ok) __nanosleep(1000000);  // copies in flight
 }
 
 // Joins the partial results of the kv rows that range boundaries cut: block i the row that holds boundary i + 1, if that is
 // the row's first.
 template <int D>
 __global__ void __launch_bounds__(256)
-kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int b0, int nb, int grid, const float* __restrict__ partial,
+kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, int b0, int nb, int grid, const float* __restrict__ partial,
                        bf16* __restrict__ out) {
   extern __shared__ int pre[];
   const int tid = threadIdx.x;
   // (the lengths are an earlier kernel's results at the latest: with the wait ahead of them everything else is too)
   pdl_wait();
-  build_prefix(W, lens, extra, b0, nb, pre, tid, 256);
+  build_prefix(W, lens, extra, chunk, b0, nb, pre, tid, 256);
   const int Hkv = W.Hkv;
   const Split sp(pre[nb] * Hkv, grid);
   const int f = ((int)blockIdx.x + 1) * sp.per;
@@ -758,13 +777,12 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int b0, int 
   const int c1 = (row1 - 1) / sp.per;
   for (int e = tid; e < G * D / 2; e += 256) {
     const int head = e / (D / 2), ch = (e % (D / 2)) * 2;
-    float mx = -INFINITY, sum = 0.f, a0 = 0.f, a1 = 0.f;
+    float mx = kLowest, sum = 0.f, a0 = 0.f, a1 = 0.f;
     for (int c = blockIdx.x; c <= c1; ++c) {
       const int slot = c == (int)blockIdx.x ? 1 : 0;  // where the row begins, and where it goes on
       const float* src = partial + ((size_t)c * 2 + slot) * partial_floats(D, G) + (size_t)head * (D + 2);
       const float2 ml = *reinterpret_cast<const float2*>(src), x = *reinterpret_cast<const float2*>(src + 2 + ch);
-      const float m2 = fmaxf(mx, ml.x), mm = m2 == -INFINITY ? 0.f : m2;
-      const float f0 = ex2(mx - mm), f1 = ex2(ml.x - mm);
+      const float m2 = fmaxf(mx, ml.x), f0 = ex2(mx - m2), f1 = ex2(ml.x - m2);
       mx = m2;
       sum = sum * f0 + ml.y * f1;
       a0 = a0 * f0 + x.x * f1;
@@ -785,7 +803,7 @@ int sm_count() {
 template <int D, int BITS, int NH>
 cudaError_t launch_token(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, float scale, float* partial,
                          bf16* out, int* status, cudaStream_t stream) {
-  using GM = TokGeom<D, BITS>;
+  using GM = TokGeom<D, BITS, NH>;
   TokMaps maps = {};
   if (BITS == 16) {
     const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)W.batch * W.Hkv * W.rows};
@@ -794,15 +812,18 @@ cudaError_t launch_token(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Te
     if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box))
       return cudaErrorInvalidValue;
   }
+  constexpr int kSmemLimit = kSmemPerSm / GM::kCtas - 1024;
   auto kern = kvm_window_token_kernel<D, BITS, NH>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemBytes - 1024);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
-  const int sms = sm_count();
-  const int max_chunks = (W.rows + kChunk - 1) / kChunk;
-  for (int b0 = 0; b0 < W.batch; b0 += kMaxBatch) {
-    const int nb = std::min(kMaxBatch, W.batch - b0);
-    int stages = 1;
-    while (stages < kMaxStages && TokSmem(GM::kStageKv, D, G, nb, stages + 1).total <= kMaxSmemBytes - 1024) ++stages;
+  const int sms = sm_count() * GM::kCtas;
+  const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
+  int per_launch = kMaxBatch;  // sequences whose lengths fit beside two stages
+  while (per_launch > 16 && TokSmem(GM::kStageKv, D, G, per_launch, 2).total > kSmemLimit) per_launch -= 16;
+  for (int b0 = 0; b0 < W.batch; b0 += per_launch) {
+    const int nb = std::min(per_launch, W.batch - b0);
+    int stages = 2;
+    while (stages < kMaxStages && TokSmem(GM::kStageKv, D, G, nb, stages + 1).total <= kSmemLimit) ++stages;
     // Whole kv rows per CTA where cutting them gains less than the second launch and the partial results cost (about
     // 2.5 us; a chunk streams in about its bytes / 44 GB/s per SM).
     const long long rows = (long long)nb * W.Hkv, chunks = rows * max_chunks;
@@ -810,12 +831,12 @@ cudaError_t launch_token(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Te
     const bool whole = (double)((rows + sms - 1) / sms) * max_chunks * chunk_us <= (double)((chunks + sms - 1) / sms) * chunk_us + 2.5;
     const int grid = (int)std::min<long long>(sms, whole ? rows : chunks);
     const TokSmem lay(GM::kStageKv, D, G, nb, stages);
-    cudaError_t err = launch_pdl(kern, dim3(grid), dim3(kTokThreads), lay.total, stream, true, W, G, q, k_new, v_new, lens, b0, nb, stages,
+    cudaError_t err = launch_pdl(kern, dim3(grid), dim3(GM::kThreads), lay.total, stream, true, W, G, q, k_new, v_new, lens, b0, nb, stages,
                                  whole ? 1 : 0, scale * kLog2e, partial, out, status, maps);
     if (err != cudaSuccess) return err;
     if (!whole && grid > 1) {
       err = launch_pdl(kvm_window_join_kernel<D>, dim3(grid - 1), dim3(256), (2 * nb + 1) * 4, stream, true, W, G, lens,
-                       k_new.ptr ? 1 : 0, b0, nb, grid, (const float*)partial, out);
+                       k_new.ptr ? 1 : 0, GM::kChunk, b0, nb, grid, (const float*)partial, out);
       if (err != cudaSuccess) return err;
     }
   }
@@ -831,7 +852,7 @@ cudaError_t launch_token_nh(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new,
 
 }  // namespace
 
-size_t window_token_workspace(int D, int G) { return (size_t)sm_count() * 2 * partial_floats(D, G) * 4; }
+size_t window_token_workspace(int D, int G) { return (size_t)sm_count() * 2 * 2 * partial_floats(D, G) * 4; }
 
 cudaError_t window_token_dispatch(int D, int bits, const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens,
                                   float scale, float* partial, bf16* out, int* status, cudaStream_t stream) {
