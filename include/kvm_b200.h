@@ -454,8 +454,15 @@ size_t kvm_window_cache_bytes(const kvm_window_cache* cache);
  * first `length` are taken.  positions_dev / lengths_dev: int32 [batch] on the device, or NULL: `position` / `length` for all
  * sequences.  A negative position, or a length of 0, leaves the sequence as it is.  Tokens that later tokens of the same
  * call push out are not written.  Positions stay below 2^31 - n_tokens. */
-int kvm_window_cache_write(const kvm_window_cache* cache, kvm_tensor4 k, kvm_tensor4 v, int64_t n_tokens, const int32_t* positions_dev,
-                           int32_t position, const int32_t* lengths_dev, int32_t length, void* stream);
+typedef struct kvm_window_write_args {
+  const kvm_window_cache* cache;
+  kvm_tensor4 k, v;
+  const int32_t* positions_dev;
+  const int32_t* lengths_dev;
+  int64_t n_tokens;
+  int32_t position, length;
+} kvm_window_write_args;
+int kvm_window_cache_write(const kvm_window_write_args* args, void* stream);
 
 /* What the cache holds of sequences of `length` tokens, in order: k_out, v_out bf16 [batch, n_kv_heads, sinks + window, head_dim],
  * the first sinks tokens, then the last `window`, zeros behind them. */
@@ -464,19 +471,34 @@ int kvm_window_cache_read(const kvm_window_cache* cache, const int32_t* lengths_
 /* One query per sequence: q [batch, n_q_heads, 1, head_dim], out bf16 [batch, n_q_heads * head_dim]; at most 16 query heads per
  * kv head.  Without a new token (k_new.ptr and v_new.ptr NULL) lengths are the tokens of the sequences, the query's own among
  * them; with one they are its positions, and it is written to the cache on the way.  A sequence of no tokens (length 0, or
- * position -1) gets zeros.  The workspace holds partial results of one call; calls in flight at the same time need one each. */
+ * position -1) gets zeros.  The workspace (none where kvm_window_attend_workspace_bytes() says 0) holds partial results of one
+ * call; calls in flight at the same time need one each.  scale > 0 multiplies the scores. */
+typedef struct kvm_window_attend_args {
+  const kvm_window_cache* cache;
+  kvm_tensor4 q, k_new, v_new;
+  const int32_t* lengths_dev;            /* int32 [batch], or NULL: `length` for all sequences */
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t n_q_heads, length;
+  float scale;
+} kvm_window_attend_args;
 size_t kvm_window_attend_workspace_bytes(const kvm_window_cache* cache, int32_t n_q_heads);
-int kvm_window_attend(const kvm_window_cache* cache, int32_t n_q_heads, kvm_tensor4 q, kvm_tensor4 k_new, kvm_tensor4 v_new,
-                      const int32_t* lengths_dev, int32_t length, float scale, void* out, void* workspace, size_t workspace_bytes,
-                      void* stream);
+int kvm_window_attend(const kvm_window_attend_args* args, void* stream);
 
 /* A prompt, or a chunk of one behind earlier tokens: q [batch, n_q_heads, n_queries, head_dim], k, v [batch, n_kv_heads, n_keys,
  * head_dim], out bf16 [batch, n_queries, n_q_heads * head_dim].  Query t stands at position n_keys - n_queries + t.
  * lengths_dev (int32 [batch], or NULL: n_keys): tokens of each sequence; tokens behind them are padding, never looked at, and
  * their output rows are zeros. */
-int kvm_window_attention(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_queries, int64_t n_keys,
-                         kvm_tensor4 q, kvm_tensor4 k, kvm_tensor4 v, int64_t window, int64_t sinks, float scale,
-                         const int32_t* lengths_dev, void* out, void* stream);
+typedef struct kvm_window_prompt_args {
+  kvm_tensor4 q, k, v;
+  const int32_t* lengths_dev;
+  void* out;
+  int64_t n_queries, n_keys, window, sinks;
+  int32_t batch, n_q_heads, n_kv_heads, head_dim;
+  float scale;
+} kvm_window_prompt_args;
+int kvm_window_attention(const kvm_window_prompt_args* args, void* stream);
 
 /* Device-side condition of the window kernels on the current device since the last call (synchronises the stream):
  * KVM_ERR_DEVICE_TIMEOUT if a bounded wait ran out.  One word per device, in the library. */

@@ -97,6 +97,27 @@ class KvmWindowCache(C.Structure):
                 ("window", C.c_int32), ("sinks", C.c_int32), ("bits", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)]
 
 
+def _tensor_fields(name):  # a kvm_tensor4, its members side by side (one assignment per call of the constructor is quicker)
+    return [(name, C.c_void_p)] + [(f"{name}_stride_{d}", C.c_int64) for d in "bht"]
+
+
+class KvmWindowWriteArgs(C.Structure):
+    _fields_ = [("cache", C.c_void_p), *_tensor_fields("k"), *_tensor_fields("v"), ("positions_dev", C.c_void_p), ("lengths_dev", C.c_void_p),
+                ("n_tokens", C.c_int64), ("position", C.c_int32), ("length", C.c_int32)]
+
+
+class KvmWindowAttendArgs(C.Structure):
+    _fields_ = [("cache", C.c_void_p), *_tensor_fields("q"), *_tensor_fields("k_new"), *_tensor_fields("v_new"), ("lengths_dev", C.c_void_p),
+                ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("n_q_heads", C.c_int32),
+                ("length", C.c_int32), ("scale", C.c_float)]
+
+
+class KvmWindowPromptArgs(C.Structure):
+    _fields_ = [*_tensor_fields("q"), *_tensor_fields("k"), *_tensor_fields("v"), ("lengths_dev", C.c_void_p), ("out", C.c_void_p),
+                ("n_queries", C.c_int64), ("n_keys", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64), ("batch", C.c_int32),
+                ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
+
+
 EXPORTS = [
     "kvm_prefill_workspace_bytes", "kvm_prefill_forward", "kvm_decode_workspace_bytes", "kvm_decode_step",
     "kvm_memory_refresh", "kvm_last_error_string", "kvm_abi_version", "kvm_decode_step_static", "kvm_prefill_status", "kvm_decode_run",
@@ -188,19 +209,13 @@ def load():
     lib.kvm_interleave_shards.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p]
     lib.kvm_window_cache_bytes.restype = C.c_size_t
     lib.kvm_window_cache_bytes.argtypes = [LP(KvmWindowCache)]
-    lib.kvm_window_cache_write.restype = C.c_int
-    lib.kvm_window_cache_write.argtypes = [LP(KvmWindowCache), KvmTensor4, KvmTensor4, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p,
-                                           C.c_int32, C.c_void_p]
+    for fn in (lib.kvm_window_cache_write, lib.kvm_window_attend, lib.kvm_window_attention):
+        fn.restype = C.c_int
+        fn.argtypes = [C.c_void_p, C.c_void_p]  # (argument blocks, by their addresses)
     lib.kvm_window_cache_read.restype = C.c_int
-    lib.kvm_window_cache_read.argtypes = [LP(KvmWindowCache), C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.kvm_window_cache_read.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.kvm_window_attend_workspace_bytes.restype = C.c_size_t
-    lib.kvm_window_attend_workspace_bytes.argtypes = [LP(KvmWindowCache), C.c_int32]
-    lib.kvm_window_attend.restype = C.c_int
-    lib.kvm_window_attend.argtypes = [LP(KvmWindowCache), C.c_int32, KvmTensor4, KvmTensor4, KvmTensor4, C.c_void_p, C.c_int32, C.c_float,
-                                      C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
-    lib.kvm_window_attention.restype = C.c_int
-    lib.kvm_window_attention.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, KvmTensor4, KvmTensor4,
-                                         KvmTensor4, C.c_int64, C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.kvm_window_attend_workspace_bytes.argtypes = [C.c_void_p, C.c_int32]
     lib.kvm_window_status.restype = C.c_int
     lib.kvm_window_status.argtypes = [C.c_void_p]
     lib.kvm_last_error_string.restype = C.c_char_p

@@ -1,5 +1,6 @@
 // extern "C" entry points of libkvm_b200: argument validation, workspace carve-up, launches.
 // Nothing here allocates device memory.  What the library keeps between calls is listed in the header.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -31,7 +32,7 @@ cudaError_t refresh_dispatch(int D, const LayerDev& L, int batch, MemoryDev mem,
 cudaError_t window_write_dispatch(int D, int bits, const WindowDev& W, Tensor4 k, Tensor4 v, int n_tokens, SeqInts positions,
                                   SeqInts lengths, cudaStream_t stream);
 cudaError_t window_read_dispatch(int D, int bits, const WindowDev& W, SeqInts lengths, bf16* k_out, bf16* v_out, cudaStream_t stream);
-size_t window_token_workspace(int D, int G);
+size_t window_token_workspace(int D, int bits, const WindowDev& W, int G);
 cudaError_t window_token_dispatch(int D, int bits, const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens,
                                   float scale, float* partial, bf16* out, int* status, cudaStream_t stream);
 cudaError_t window_prompt_dispatch(int D, int batch, int Hq, int Hkv, int T, int S, Tensor4 q, Tensor4 k, Tensor4 v, int window,
@@ -210,21 +211,20 @@ int static_scratch_for_current_device(void** out) {
 
 // ---- sliding-window operators
 __device__ int g_window_status;  // set by a window kernel whose bounded wait ran out
-int* g_window_status_ptr[kMaxDevices] = {nullptr};
+std::atomic<int*> g_window_status_ptr[kMaxDevices] = {};
 
 int window_status_word(int** out) {
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "window operators: cudaGetDevice");
   if (dev < 0 || dev >= kMaxDevices) return fail(KVM_ERR_UNSUPPORTED, "window operators: device ordinal %d not supported", dev);
-  std::lock_guard<std::mutex> lock(g_static_mu);
-  if (!g_window_status_ptr[dev]) {
-    void* p = nullptr;
-    e = cudaGetSymbolAddress(&p, g_window_status);
-    if (e != cudaSuccess) return cuda_fail(e, "window operators: cudaGetSymbolAddress");
-    g_window_status_ptr[dev] = static_cast<int*>(p);
-  }
-  *out = g_window_status_ptr[dev];
+  *out = g_window_status_ptr[dev].load(std::memory_order_acquire);
+  if (*out) return KVM_OK;
+  void* p = nullptr;
+  e = cudaGetSymbolAddress(&p, g_window_status);
+  if (e != cudaSuccess) return cuda_fail(e, "window operators: cudaGetSymbolAddress");
+  *out = static_cast<int*>(p);
+  g_window_status_ptr[dev].store(*out, std::memory_order_release);
   return KVM_OK;
 }
 
@@ -535,21 +535,22 @@ size_t kvm_window_cache_bytes(const kvm_window_cache* cache) {
 size_t kvm_window_attend_workspace_bytes(const kvm_window_cache* cache, int32_t n_q_heads) {
   g_err[0] = 0;
   if (check_window(cache, false) || check_groups(cache, n_q_heads)) return 0;
-  return window_token_workspace(cache->head_dim, n_q_heads / cache->n_kv_heads);
+  return window_token_workspace(cache->head_dim, cache->bits, window_dev(cache), n_q_heads / cache->n_kv_heads);
 }
 
-int kvm_window_cache_write(const kvm_window_cache* cache, kvm_tensor4 k, kvm_tensor4 v, int64_t n_tokens, const int32_t* positions_dev,
-                           int32_t position, const int32_t* lengths_dev, int32_t length, void* stream) {
+int kvm_window_cache_write(const kvm_window_write_args* a, void* stream) {
   g_err[0] = 0;
+  if (!a) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_cache_write: arguments must not be NULL");
+  const kvm_window_cache* cache = a->cache;
   if (int rc = check_window(cache, true)) return rc;
-  if (n_tokens < 0 || n_tokens > 0x7fffffff) return fail(KVM_ERR_BAD_ARGUMENT, "n_tokens %lld outside [0, 2^31)", (long long)n_tokens);
-  if (n_tokens == 0) return KVM_OK;
-  if (int rc = check_tensor(k, "k", cache->head_dim)) return rc;
-  if (int rc = check_tensor(v, "v", cache->head_dim)) return rc;
-  if (!positions_dev && (int64_t)position + n_tokens > 0x7fffffff)
-    return fail(KVM_ERR_BAD_ARGUMENT, "position %d: tokens beyond 2^31 - 1", position);
-  const cudaError_t e = window_write_dispatch(cache->head_dim, cache->bits, window_dev(cache), to_dev(k), to_dev(v), (int)n_tokens,
-                                              SeqInts{positions_dev, position}, SeqInts{lengths_dev, length},
+  if (a->n_tokens < 0 || a->n_tokens > 0x7fffffff) return fail(KVM_ERR_BAD_ARGUMENT, "n_tokens %lld outside [0, 2^31)", (long long)a->n_tokens);
+  if (a->n_tokens == 0) return KVM_OK;
+  if (int rc = check_tensor(a->k, "k", cache->head_dim)) return rc;
+  if (int rc = check_tensor(a->v, "v", cache->head_dim)) return rc;
+  if (!a->positions_dev && (int64_t)a->position + a->n_tokens > 0x7fffffff)
+    return fail(KVM_ERR_BAD_ARGUMENT, "position %d: tokens beyond 2^31 - 1", a->position);
+  const cudaError_t e = window_write_dispatch(cache->head_dim, cache->bits, window_dev(cache), to_dev(a->k), to_dev(a->v), (int)a->n_tokens,
+                                              SeqInts{a->positions_dev, a->position}, SeqInts{a->lengths_dev, a->length},
                                               static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kvm_window_cache_write");
   return KVM_OK;
@@ -566,62 +567,65 @@ int kvm_window_cache_read(const kvm_window_cache* cache, const int32_t* lengths_
   return KVM_OK;
 }
 
-int kvm_window_attend(const kvm_window_cache* cache, int32_t n_q_heads, kvm_tensor4 q, kvm_tensor4 k_new, kvm_tensor4 v_new,
-                      const int32_t* lengths_dev, int32_t length, float scale, void* out, void* workspace, size_t workspace_bytes,
-                      void* stream) {
+int kvm_window_attend(const kvm_window_attend_args* a, void* stream) {
   g_err[0] = 0;
+  if (!a) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: arguments must not be NULL");
+  const kvm_window_cache* cache = a->cache;
   if (int rc = check_window(cache, true)) return rc;
-  if (int rc = check_groups(cache, n_q_heads)) return rc;
-  if (int rc = check_tensor(q, "q", cache->head_dim)) return rc;
-  if ((k_new.ptr == nullptr) != (v_new.ptr == nullptr)) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: k and v of the new token go together");
-  if (k_new.ptr) {
-    if (int rc = check_tensor(k_new, "k", cache->head_dim)) return rc;
-    if (int rc = check_tensor(v_new, "v", cache->head_dim)) return rc;
+  if (int rc = check_groups(cache, a->n_q_heads)) return rc;
+  if (int rc = check_tensor(a->q, "q", cache->head_dim)) return rc;
+  if ((a->k_new.ptr == nullptr) != (a->v_new.ptr == nullptr))
+    return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: k and v of the new token go together");
+  if (a->k_new.ptr) {
+    if (int rc = check_tensor(a->k_new, "k", cache->head_dim)) return rc;
+    if (int rc = check_tensor(a->v_new, "v", cache->head_dim)) return rc;
   }
-  if (int rc = check_scale(scale)) return rc;
-  if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: out must be 16-byte aligned and not NULL");
-  const int G = n_q_heads / cache->n_kv_heads;
-  if (!workspace || ((uintptr_t)workspace) % 16 || workspace_bytes < window_token_workspace(cache->head_dim, G))
-    return fail(KVM_ERR_CAPACITY, "kvm_window_attend: workspace of %zu bytes (needs %zu, 16-byte aligned)", workspace_bytes,
-                window_token_workspace(cache->head_dim, G));
+  if (int rc = check_scale(a->scale)) return rc;
+  if (!a->out || ((uintptr_t)a->out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: out must be 16-byte aligned and not NULL");
+  const int G = a->n_q_heads / cache->n_kv_heads;
+  const WindowDev w = window_dev(cache);
+  const size_t need = window_token_workspace(cache->head_dim, cache->bits, w, G);
+  if (need && (!a->workspace || ((uintptr_t)a->workspace) % 16 || a->workspace_bytes < need))
+    return fail(KVM_ERR_CAPACITY, "kvm_window_attend: workspace of %zu bytes (needs %zu, 16-byte aligned)", a->workspace_bytes, need);
   int* status = nullptr;
   if (int rc = window_status_word(&status)) return rc;
-  const cudaError_t e = window_token_dispatch(cache->head_dim, cache->bits, window_dev(cache), G, to_dev(q), to_dev(k_new), to_dev(v_new),
-                                              SeqInts{lengths_dev, length}, scale, static_cast<float*>(workspace),
-                                              static_cast<bf16*>(out), status, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = window_token_dispatch(cache->head_dim, cache->bits, w, G, to_dev(a->q), to_dev(a->k_new), to_dev(a->v_new),
+                                              SeqInts{a->lengths_dev, a->length}, a->scale, static_cast<float*>(a->workspace),
+                                              static_cast<bf16*>(a->out), status, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kvm_window_attend");
   return KVM_OK;
 }
 
-int kvm_window_attention(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_queries, int64_t n_keys,
-                         kvm_tensor4 q, kvm_tensor4 k, kvm_tensor4 v, int64_t window, int64_t sinks, float scale,
-                         const int32_t* lengths_dev, void* out, void* stream) {
+int kvm_window_attention(const kvm_window_prompt_args* a, void* stream) {
   g_err[0] = 0;
-  if (head_dim != 32 && head_dim != 64 && head_dim != 128) return fail(KVM_ERR_UNSUPPORTED, "head_dim %d not supported (32, 64 or 128)", head_dim);
-  if (n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
-    return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, n_kv_heads);
-  if (batch < 0 || n_queries < 0 || n_keys < n_queries || n_keys > 0x3fffffff)
-    return fail(KVM_ERR_BAD_ARGUMENT, "batch %d, %lld queries, %lld keys: none negative, at least as many keys as queries, below 2^30", batch,
-                (long long)n_queries, (long long)n_keys);
-  if (window < 1 || sinks < 0) return fail(KVM_ERR_BAD_ARGUMENT, "window %lld must be at least 1, sinks %lld not negative", (long long)window, (long long)sinks);
-  if (batch == 0 || n_queries == 0) return KVM_OK;
-  if (int rc = check_tensor(q, "q", head_dim)) return rc;
-  if (int rc = check_tensor(k, "k", head_dim)) return rc;
-  if (int rc = check_tensor(v, "v", head_dim)) return rc;
-  if (int rc = check_scale(scale)) return rc;
+  if (!a) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: arguments must not be NULL");
+  if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128)
+    return fail(KVM_ERR_UNSUPPORTED, "head_dim %d not supported (32, 64 or 128)", a->head_dim);
+  if (a->n_kv_heads <= 0 || a->n_q_heads <= 0 || a->n_q_heads % a->n_kv_heads)
+    return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", a->n_q_heads, a->n_kv_heads);
+  if (a->batch < 0 || a->n_queries < 0 || a->n_keys < a->n_queries || a->n_keys > 0x3fffffff)
+    return fail(KVM_ERR_BAD_ARGUMENT, "batch %d, %lld queries, %lld keys: none negative, at least as many keys as queries, below 2^30",
+                a->batch, (long long)a->n_queries, (long long)a->n_keys);
+  if (a->window < 1 || a->sinks < 0)
+    return fail(KVM_ERR_BAD_ARGUMENT, "window %lld must be at least 1, sinks %lld not negative", (long long)a->window, (long long)a->sinks);
+  if (int rc = check_scale(a->scale)) return rc;
+  if (a->batch == 0 || a->n_queries == 0) return KVM_OK;
+  if (int rc = check_tensor(a->q, "q", a->head_dim)) return rc;
+  if (int rc = check_tensor(a->k, "k", a->head_dim)) return rc;
+  if (int rc = check_tensor(a->v, "v", a->head_dim)) return rc;
   // (the copies step by the strides: an expanded dimension is the caller's to lay out)
-  const kvm_tensor4* in[3] = {&q, &k, &v};
+  const kvm_tensor4* in[3] = {&a->q, &a->k, &a->v};
   for (int i = 0; i < 3; ++i)
-    if ((batch > 1 && in[i]->stride_b <= 0) || ((i ? n_kv_heads : n_q_heads) > 1 && in[i]->stride_h <= 0) ||
-        ((i ? n_keys : n_queries) > 1 && in[i]->stride_t <= 0))
+    if ((a->batch > 1 && in[i]->stride_b <= 0) || ((i ? a->n_kv_heads : a->n_q_heads) > 1 && in[i]->stride_h <= 0) ||
+        ((i ? a->n_keys : a->n_queries) > 1 && in[i]->stride_t <= 0))
       return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: strides must be positive");
-  if (!out || ((uintptr_t)out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must be 16-byte aligned and not NULL");
+  if (!a->out || ((uintptr_t)a->out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must be 16-byte aligned and not NULL");
   int* status = nullptr;
   if (int rc = window_status_word(&status)) return rc;
-  const int w = (int)(window < n_keys ? window : n_keys), s = (int)(sinks < n_keys ? sinks : n_keys);
-  const cudaError_t e = window_prompt_dispatch(head_dim, batch, n_q_heads, n_kv_heads, (int)n_queries, (int)n_keys, to_dev(q), to_dev(k),
-                                               to_dev(v), w, s, scale, lengths_dev, static_cast<bf16*>(out), status,
-                                               static_cast<cudaStream_t>(stream));
+  const int w = (int)(a->window < a->n_keys ? a->window : a->n_keys), s = (int)(a->sinks < a->n_keys ? a->sinks : a->n_keys);
+  const cudaError_t e = window_prompt_dispatch(a->head_dim, a->batch, a->n_q_heads, a->n_kv_heads, (int)a->n_queries, (int)a->n_keys,
+                                               to_dev(a->q), to_dev(a->k), to_dev(a->v), w, s, a->scale, a->lengths_dev,
+                                               static_cast<bf16*>(a->out), status, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kvm_window_attention");
   return KVM_OK;
 }

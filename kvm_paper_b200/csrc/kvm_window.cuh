@@ -20,6 +20,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kvm_common.cuh"
 #include "kvm_pdl.cuh"
 #include "kvm_tc.cuh"
@@ -87,6 +89,30 @@ __device__ __forceinline__ void e2m1_to_f16x2(uint32_t w, uint32_t& o0, uint32_t
       "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
       : "=r"(o0), "=r"(o1), "=r"(o2), "=r"(o3)
       : "r"(w));
+}
+
+// What does not change between launches on a device, asked for once (device ordinals below 64, checked where the calls enter).
+inline int window_sm_count() {
+  static std::atomic<int> count[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    count[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+// Raises a kernel's limit of dynamic shared memory, once per device (`done`: the kernel's own bits).
+template <typename F>
+inline cudaError_t raise_smem_limit(F kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (done.load(std::memory_order_acquire) >> (dev & 63) & 1) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(1ull << (dev & 63), std::memory_order_release);
+  return e;
 }
 
 }  // namespace kvm

@@ -587,7 +587,8 @@ bool encode_rows(CUtensorMap* m, const Tensor4& t, int batch, int heads, int row
 template <int DP>
 cudaError_t launch_prompt(const PromptArgs& a, int sms, cudaStream_t stream) {
   auto kern = kvm_window_prompt_kernel<DP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PC<DP>::kSmem);
+  static std::atomic<unsigned long long> raised{0};
+  const cudaError_t e = raise_smem_limit(kern, PC<DP>::kSmem, raised);
   if (e != cudaSuccess) return e;
   // the register split draws on what the block is launched with
   static const bool regs_ok = [&] {
@@ -617,8 +618,7 @@ cudaError_t window_prompt_dispatch(int D, int batch, int Hq, int Hkv, int T, int
   if (!encode_rows(&a.mq, q, batch, Hq, T, D, &a.q_head_inner) || !encode_rows(&a.mk, k, batch, Hkv, S, D, &a.k_head_inner) ||
       !encode_rows(&a.mv, v, batch, Hkv, S, D, &a.v_head_inner))
     return cudaErrorInvalidValue;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+  const int sms = window_sm_count();
   return D == 128 ? launch_prompt<128>(a, sms, stream) : launch_prompt<64>(a, sms, stream);
 }
 

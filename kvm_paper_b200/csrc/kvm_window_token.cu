@@ -16,6 +16,7 @@
 // largest value.
 // The new token: the CTA that reads the chunk with its row patches the stage and writes the row to memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "kvm_tma_host.cuh"
 #include "kvm_window.cuh"
@@ -794,72 +795,96 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
 
 namespace {
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  return n;
-}
+// How a call of nb sequences is launched.
+struct TokPlan {
+  // sequences whose lengths fit beside two stages
+  template <typename GM>
+  static int sequences(int D, int G, int limit) {
+    int n = kMaxBatch;
+    while (n > 16 && TokSmem(GM::kStageKv, D, G, n, 2).total > limit) n -= 16;
+    return n;
+  }
+  // Whole kv rows per CTA where cutting them gains less than the second launch and the partial results cost (about 2.5 us;
+  // a chunk streams in about its bytes / 44 GB/s per SM).
+  template <typename GM>
+  static bool whole_rows(const WindowDev& W, int nb, int ctas) {
+    const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
+    const long long rows = (long long)nb * W.Hkv, chunks = rows * max_chunks;
+    const double chunk_us = GM::kStageKv / 44e3 * GM::kCtas;
+    return (double)((rows + ctas - 1) / ctas) * max_chunks * chunk_us <= (double)((chunks + ctas - 1) / ctas) * chunk_us + 2.5;
+  }
+};
 
 template <int D, int BITS, int NH>
-cudaError_t launch_token(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, float scale, float* partial,
-                         bf16* out, int* status, cudaStream_t stream) {
+struct TokLaunch {
   using GM = TokGeom<D, BITS, NH>;
-  TokMaps maps = {};
-  if (BITS == 16) {
-    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)W.batch * W.Hkv * W.rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)GM::kBoxW, (cuuint32_t)kBox};
-    if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box))
-      return cudaErrorInvalidValue;
-  }
-  constexpr int kSmemLimit = kSmemPerSm / GM::kCtas - 1024;
-  auto kern = kvm_window_token_kernel<D, BITS, NH>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
-  if (e != cudaSuccess) return e;
-  const int sms = sm_count() * GM::kCtas;
-  const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
-  int per_launch = kMaxBatch;  // sequences whose lengths fit beside two stages
-  while (per_launch > 16 && TokSmem(GM::kStageKv, D, G, per_launch, 2).total > kSmemLimit) per_launch -= 16;
-  for (int b0 = 0; b0 < W.batch; b0 += per_launch) {
-    const int nb = std::min(per_launch, W.batch - b0);
-    int stages = 2;
-    while (stages < kMaxStages && TokSmem(GM::kStageKv, D, G, nb, stages + 1).total <= kSmemLimit) ++stages;
-    // Whole kv rows per CTA where cutting them gains less than the second launch and the partial results cost (about
-    // 2.5 us; a chunk streams in about its bytes / 44 GB/s per SM).
-    const long long rows = (long long)nb * W.Hkv, chunks = rows * max_chunks;
-    const double chunk_us = GM::kStageKv / 44e3;
-    const bool whole = (double)((rows + sms - 1) / sms) * max_chunks * chunk_us <= (double)((chunks + sms - 1) / sms) * chunk_us + 2.5;
-    const int grid = (int)std::min<long long>(sms, whole ? rows : chunks);
-    const TokSmem lay(GM::kStageKv, D, G, nb, stages);
-    cudaError_t err = launch_pdl(kern, dim3(grid), dim3(GM::kThreads), lay.total, stream, true, W, G, q, k_new, v_new, lens, b0, nb, stages,
-                                 whole ? 1 : 0, scale * kLog2e, partial, out, status, maps);
-    if (err != cudaSuccess) return err;
-    if (!whole && grid > 1) {
-      err = launch_pdl(kvm_window_join_kernel<D>, dim3(grid - 1), dim3(256), (2 * nb + 1) * 4, stream, true, W, G, lens,
-                       k_new.ptr ? 1 : 0, GM::kChunk, b0, nb, grid, (const float*)partial, out);
-      if (err != cudaSuccess) return err;
-    }
-  }
-  return cudaSuccess;
-}
+  static constexpr int kSmemLimit = kSmemPerSm / GM::kCtas - 1024;
 
-template <int D, int BITS>
-cudaError_t launch_token_nh(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, float scale, float* partial,
-                            bf16* out, int* status, cudaStream_t stream) {
-  return G <= 8 ? launch_token<D, BITS, 1>(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream)
-                : launch_token<D, BITS, 2>(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream);
+  static size_t workspace(const WindowDev& W, int G) {
+    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(D, G, kSmemLimit);
+    for (int b0 = 0; b0 < W.batch; b0 += per)
+      if (!TokPlan::whole_rows<GM>(W, std::min(per, W.batch - b0), ctas)) return (size_t)ctas * 2 * partial_floats(D, G) * 4;
+    return 0;
+  }
+
+  static cudaError_t run(const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, float scale, float* partial,
+                         bf16* out, int* status, cudaStream_t stream) {
+    TokMaps maps;
+    if (BITS == 16) {
+      const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)W.batch * W.Hkv * W.rows};
+      const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+      const cuuint32_t box[2] = {(cuuint32_t)GM::kBoxW, (cuuint32_t)kBox};
+      if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box))
+        return cudaErrorInvalidValue;
+    }
+    auto kern = kvm_window_token_kernel<D, BITS, NH>;
+    static std::atomic<unsigned long long> raised{0};
+    cudaError_t e = raise_smem_limit(kern, kSmemLimit, raised);
+    if (e != cudaSuccess) return e;
+    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(D, G, kSmemLimit);
+    const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
+    for (int b0 = 0; b0 < W.batch; b0 += per) {
+      const int nb = std::min(per, W.batch - b0);
+      int stages = 2;
+      while (stages < kMaxStages && TokSmem(GM::kStageKv, D, G, nb, stages + 1).total <= kSmemLimit) ++stages;
+      const bool whole = TokPlan::whole_rows<GM>(W, nb, ctas);
+      const long long rows = (long long)nb * W.Hkv;
+      const int grid = (int)std::min<long long>(ctas, whole ? rows : rows * max_chunks);
+      e = launch_pdl(kern, dim3(grid), dim3(GM::kThreads), TokSmem(GM::kStageKv, D, G, nb, stages).total, stream, true, W, G, q, k_new, v_new,
+                     lens, b0, nb, stages, whole ? 1 : 0, scale * kLog2e, partial, out, status, maps);
+      if (e != cudaSuccess) return e;
+      if (!whole && grid > 1) {
+        e = launch_pdl(kvm_window_join_kernel<D>, dim3(grid - 1), dim3(256), (2 * nb + 1) * 4, stream, true, W, G, lens, k_new.ptr ? 1 : 0,
+                       GM::kChunk, b0, nb, grid, (const float*)partial, out);
+        if (e != cudaSuccess) return e;
+      }
+    }
+    return cudaSuccess;
+  }
+};
+
+template <typename F>
+auto token_variant(int D, int bits, int G, F f) {
+  auto heads = [&](auto d, auto b) {
+    constexpr int kD = decltype(d)::value, kB = decltype(b)::value;
+    return G <= 8 ? f(TokLaunch<kD, kB, 1>{}) : f(TokLaunch<kD, kB, 2>{});
+  };
+  auto width = [&](auto b) {
+    return D == 128 ? heads(std::integral_constant<int, 128>{}, b)
+                    : D == 64 ? heads(std::integral_constant<int, 64>{}, b) : heads(std::integral_constant<int, 32>{}, b);
+  };
+  return bits == 4 ? width(std::integral_constant<int, 4>{}) : width(std::integral_constant<int, 16>{});
 }
 
 }  // namespace
 
-size_t window_token_workspace(int D, int G) { return (size_t)sm_count() * 2 * 2 * partial_floats(D, G) * 4; }
+size_t window_token_workspace(int D, int bits, const WindowDev& W, int G) {
+  return token_variant(D, bits, G, [&](auto v) { return v.workspace(W, G); });
+}
 
 cudaError_t window_token_dispatch(int D, int bits, const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens,
                                   float scale, float* partial, bf16* out, int* status, cudaStream_t stream) {
-#define KVM_TOKEN(d) (bits == 4 ? launch_token_nh<d, 4>(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream) \
-                                : launch_token_nh<d, 16>(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream))
-  return D == 128 ? KVM_TOKEN(128) : D == 64 ? KVM_TOKEN(64) : KVM_TOKEN(32);
-#undef KVM_TOKEN
+  return token_variant(D, bits, G, [&](auto v) { return v.run(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream); });
 }
 
 }  // namespace kvm

@@ -23,40 +23,48 @@ import math
 import torch
 
 from . import _lib
-from ._lib import KvmTensor4
 from .ops import _stream_ptr
 
 MAX_GROUP = 16  # query heads per kv head of the single-token calls
+_BF16 = torch.bfloat16
 
 
-def _rows(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
-    """[B,H,T,D] bf16 rows that are contiguous and start on 16-byte boundaries: a view where that is so already."""
-    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
+def _rows(t: torch.Tensor, name: str, shape, dev) -> tuple:
+    """[B,H,T,D] bf16 rows that are contiguous and start on 16-byte boundaries, as they lie in memory where that is so
+    already: (address, strides of B, H and T, the tensor that holds them)."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape) if isinstance(t, torch.Tensor) else type(t)}")
-    if t.dtype is not torch.bfloat16:
+    if t.dtype is not _BF16:
         raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must live on a CUDA device (there is no CPU path)")
     if t.device != dev:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must live on a CUDA device (there is no CPU path)")
         raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
-    if torch.is_grad_enabled() and t.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("the window operators implement inference only; call them under torch.no_grad()")
-    st = t.stride()
-    # (a dimension of one entry is never stepped over)
-    if st[3] != 1 or t.data_ptr() % 16 or any(s % 8 or s <= 0 for s, n in zip(st[:3], t.shape) if n > 1):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    b, h, r, d = t.stride()
+    p = t.data_ptr()
+    if d != 1 or p & 15 or (b | h | r) & 7 or b <= 0 or h <= 0 or r <= 0:
+        # a dimension of one entry is never stepped over: any stride will do there
+        full = shape[3]
+        b, h, r = (s if n > 1 else full for s, n in zip((b, h, r), shape))
+        if (d != 1 and full > 1) or p & 15 or (b | h | r) & 7 or b <= 0 or h <= 0 or r <= 0:
+            t = t.clone(memory_format=torch.contiguous_format)
+            b, h, r, _ = t.stride()
+            p = t.data_ptr()
+    return p, b, h, r, t
 
 
-def _arg(t: torch.Tensor) -> KvmTensor4:
-    st = t.stride()
-    return KvmTensor4(t.data_ptr(), *(s if n > 1 else 0 for s, n in zip(st[:3], t.shape)))
+def _shape4(t, name: str, want: str):
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise ValueError(f"{name} must be a {want} tensor, got {list(t.shape) if isinstance(t, torch.Tensor) else type(t)}")
+    return t.shape
 
 
 def _counts(x, name: str, batch: int, dev, least: int, most: int):
     """(device address or None, number for all) of per-sequence positions or lengths."""
     if isinstance(x, torch.Tensor):
-        if x.dtype is not torch.int32 or tuple(x.shape) != (batch,) or not x.is_contiguous():
+        if x.dtype is not torch.int32 or x.shape != (batch,) or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of {batch} entries, got {tuple(x.shape)} {x.dtype}")
         if x.device != dev:
             raise RuntimeError(f"{name} must be on {dev}, got {x.device}")
@@ -67,17 +75,17 @@ def _counts(x, name: str, batch: int, dev, least: int, most: int):
     return None, x
 
 
-def _output(out, shape, dev) -> torch.Tensor:
+def _output(out, like: torch.Tensor, shape) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, device=dev, dtype=torch.bfloat16)
-    if tuple(out.shape) != tuple(shape) or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned bf16 tensor {list(shape)} on {dev}, got {list(out.shape)} {out.dtype}")
+        return like.new_empty(shape)
+    if out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous() or out.device != like.device or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned bf16 tensor {list(shape)} on {like.device}, got {list(out.shape)} {out.dtype}")
     return out
 
 
 def _scale(scale, head_dim: int) -> float:
     s = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not 0.0 < s < math.inf:
+    if not 0.0 < s < 3e38:
         raise ValueError(f"scale must be positive and finite, got {s}")
     return s
 
@@ -102,22 +110,21 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ``window - 1`` tokens are there.)  ``window`` None: every earlier token is visible.  ``lengths`` (int32 [B]): tokens of each
     sequence, S at most; what lies behind them is padding, is never looked at, and its output rows are zeros.
     Returns [B,T,Hq*D] (``out`` if given)."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor) or t.dim() != 4:
-            raise ValueError(f"{name} must be a [B,H,T,D] tensor, got {list(t.shape) if isinstance(t, torch.Tensor) else type(t)}")
-    B, Hq, T, D = q.shape
-    Hkv, S = k.size(1), k.size(2)
+    B, Hq, T, D = _shape4(q, "q", "[B,Hq,T,D]")
+    _, Hkv, S, _ = _shape4(k, "k", "[B,Hkv,S,D]")
     dev = q.device
-    window = max(S, 1) if window is None else int(window)
-    q, k, v = _rows(q, "q", (B, Hq, T, D), dev), _rows(k, "k", (B, Hkv, S, D), dev), _rows(v, "v", (B, Hkv, S, D), dev)
-    sc = _scale(scale, D)
+    if not q.is_cuda:
+        raise RuntimeError("kvm_b200 runs on CUDA tensors only (there is no CPU path)")
+    qa, ka, va = _rows(q, "q", (B, Hq, T, D), dev), _rows(k, "k", (B, Hkv, S, D), dev), _rows(v, "v", (B, Hkv, S, D), dev)
     lens = None
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor):
             raise ValueError(f"lengths must be an int32 tensor, got {type(lengths)}")
         lens, _ = _counts(lengths, "lengths", B, dev, 0, S)
-    y = _output(out, (B, T, Hq * D), dev)
-    _call(dev, _lib.load().kvm_window_attention, B, Hq, Hkv, D, T, S, _arg(q), _arg(k), _arg(v), window, int(sinks), sc, lens, y.data_ptr())
+    y = _output(out, q, (B, T, Hq * D))
+    args = _lib.KvmWindowPromptArgs(*qa[:4], *ka[:4], *va[:4], lens, y.data_ptr(), T, S, max(S, 1) if window is None else int(window),
+                                    int(sinks), B, Hq, Hkv, D, _scale(scale, D))
+    _call(dev, _lib.load().kvm_window_attention, C.addressof(args))
     return y
 
 
@@ -141,73 +148,81 @@ class WindowCache:
             raise ValueError(lib.kvm_last_error_string().decode())
         self.device = dev = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
         self.rows = -(-self.sinks // 16) * 16 + -(-self.window // 16) * 16
-        self.k = self.v = self._blocks = None
+        self._k = self._v = self._blocks = None
         if self.bits == 4:
             self._blocks = torch.zeros(n, device=dev, dtype=torch.uint8)
             c.k = self._blocks.data_ptr()
         else:  # rows in the cache's own order: sinks first, then the ring
             shape = (self.batch, self.n_kv_heads, self.rows, self.head_dim)
-            self.k, self.v = (torch.zeros(shape, device=dev, dtype=torch.bfloat16) for _ in range(2))
-            c.k, c.v = self.k.data_ptr(), self.v.data_ptr()
-        self._arg = C.byref(c)
+            self._k, self._v = (torch.zeros(shape, device=dev, dtype=_BF16) for _ in range(2))
+            c.k, c.v = self._k.data_ptr(), self._v.data_ptr()
+        self._addr = C.addressof(c)
         self._workspace_bytes: dict[int, int] = {}
 
+    @property
+    def k(self) -> torch.Tensor | None:
+        """Keys of a 16-bit cache [B,Hkv,rows,D] in the cache's own order (include/kvm_b200.h); None for 4 bits (``read``)."""
+        return self._k
+
+    @property
+    def v(self) -> torch.Tensor | None:
+        """Values, as ``k``."""
+        return self._v
+
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self._blocks) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (self._k, self._v, self._blocks) if t is not None)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, positions, lengths=None) -> None:
         """Writes tokens ``positions[b] ...`` of every sequence: k, v [B,Hkv,T,D], of which sequence b brings the first
         ``lengths[b]`` (None: all).  A negative position leaves its sequence as it is.  Positions stay below 2^31 - T.  Tokens that
         later ones of the call push out are not written."""
-        if not isinstance(k, torch.Tensor) or k.dim() != 4:
-            raise ValueError(f"k must be a [B,Hkv,T,D] tensor, got {list(k.shape) if isinstance(k, torch.Tensor) else type(k)}")
-        shape = (self.batch, self.n_kv_heads, k.size(2), self.head_dim)
-        k, v = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
-        T = shape[2]
-        p = _counts(positions, "positions", self.batch, self.device, -1, 2**31 - 1 - T)
-        n = _counts(T if lengths is None else lengths, "lengths", self.batch, self.device, 0, T)
-        _call(self.device, _lib.load().kvm_window_cache_write, self._arg, _arg(k), _arg(v), T, *p, *n)
+        T = _shape4(k, "k", "[B,Hkv,T,D]")[2]
+        shape = (self.batch, self.n_kv_heads, T, self.head_dim)
+        ka, va = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
+        p, p_all = _counts(positions, "positions", self.batch, self.device, -1, 2**31 - 1 - T)
+        n, n_all = (None, T) if lengths is None else _counts(lengths, "lengths", self.batch, self.device, 0, T)
+        args = _lib.KvmWindowWriteArgs(self._addr, *ka[:4], *va[:4], p, n, T, p_all, n_all)
+        _call(self.device, _lib.load().kvm_window_cache_write, C.addressof(args))
 
     def read(self, lengths) -> tuple[torch.Tensor, torch.Tensor]:
         """What the cache holds of sequences of ``lengths`` tokens, in order: (k, v) [B,Hkv,sinks+window,D], the first sinks
         tokens, then the last ``window`` ones; zeros behind the last token."""
-        n = _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1)
-        shape = (self.batch, self.n_kv_heads, self.sinks + self.window, self.head_dim)
-        k, v = (torch.empty(shape, device=self.device, dtype=torch.bfloat16) for _ in range(2))
-        _call(self.device, _lib.load().kvm_window_cache_read, self._arg, *n, k.data_ptr(), v.data_ptr())
+        n, n_all = _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1)
+        kv = torch.empty((2, self.batch, self.n_kv_heads, self.sinks + self.window, self.head_dim), device=self.device, dtype=_BF16)
+        k, v = kv.unbind(0)
+        _call(self.device, _lib.load().kvm_window_cache_read, self._addr, n, n_all, k.data_ptr(), v.data_ptr())
         return k, v
 
-    def _attend(self, q, new, counts, scale, out):
-        if not isinstance(q, torch.Tensor) or q.dim() != 4:
-            raise ValueError(f"q must be a [B,Hq,1,D] tensor, got {list(q.shape) if isinstance(q, torch.Tensor) else type(q)}")
-        dev, Hq = self.device, q.size(1)
-        q = _rows(q, "q", (self.batch, Hq, 1, self.head_dim), dev)
+    def _attend(self, q, ka, va, counts, scale, out):
+        Hq = _shape4(q, "q", "[B,Hq,1,D]")[1]
+        qa = _rows(q, "q", (self.batch, Hq, 1, self.head_dim), self.device)
         lib = _lib.load()
         need = self._workspace_bytes.get(Hq)
         if need is None:
             if Hq <= 0 or Hq % self.n_kv_heads or Hq // self.n_kv_heads > MAX_GROUP:
                 raise ValueError(f"{Hq} query heads over {self.n_kv_heads} kv heads: a multiple of them, at most {MAX_GROUP} each")
-            need = self._workspace_bytes[Hq] = lib.kvm_window_attend_workspace_bytes(self._arg, Hq)
-        y = _output(out, (self.batch, 1, Hq * self.head_dim), dev)
+            need = self._workspace_bytes[Hq] = lib.kvm_window_attend_workspace_bytes(self._addr, Hq)
+        y = _output(out, q, (self.batch, 1, Hq * self.head_dim))
         # partial results: of this call alone (calls on two streams, or in two captured graphs, do not share them)
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-        none = KvmTensor4(None, 0, 0, 0)
-        kn, vn = (_arg(t) for t in new) if new else (none, none)
-        _call(dev, lib.kvm_window_attend, self._arg, Hq, _arg(q), kn, vn, *counts, _scale(scale, self.head_dim), y.data_ptr(), ws.data_ptr(), need)
+        ws = q.new_empty(need >> 1) if need else None
+        args = _lib.KvmWindowAttendArgs(self._addr, *qa[:4], *ka, *va, counts[0], y.data_ptr(), ws.data_ptr() if need else None, need, Hq,
+                                        counts[1], _scale(scale, self.head_dim))
+        _call(self.device, lib.kvm_window_attend, C.addressof(args))
         return y
 
     def attend(self, q: torch.Tensor, lengths, *, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """One query per sequence over the cached tokens: q [B,Hq,1,D], ``lengths`` the tokens of the sequences, the query's own
         among them.  Returns [B,1,Hq*D]; a sequence of no tokens gets zeros."""
-        return self._attend(q, None, _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1), scale, out)
+        none = (None, 0, 0, 0)
+        return self._attend(q, none, none, _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1), scale, out)
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions, *, scale: float | None = None,
              out: torch.Tensor | None = None) -> torch.Tensor:
         """``write`` of one token per sequence (k, v [B,Hkv,1,D]) at ``positions`` and ``attend`` of its query in one pass.  A
         sequence at position -1 is left alone and gets zeros."""
         shape = (self.batch, self.n_kv_heads, 1, self.head_dim)
-        new = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
-        return self._attend(q, new, _counts(positions, "positions", self.batch, self.device, -1, 2**31 - 2), scale, out)
+        ka, va = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
+        return self._attend(q, ka[:4], va[:4], _counts(positions, "positions", self.batch, self.device, -1, 2**31 - 2), scale, out)
 
 
 def check_status(device="cuda") -> None:
