@@ -41,7 +41,7 @@ struct TokGeom {
   static constexpr int kChunk = kMathWarps * 16 * kTiles;        // rows per chunk
   static constexpr bool kProducer = BITS == 16;
   static constexpr int kThreads = (kMathWarps + (kProducer ? 1 : 0)) * 32;
-  static constexpr int kCtas = BITS == 4 && NH == 1 ? 2 : 1;     // per SM
+  static constexpr int kCtas = BITS == 4 && D * NH <= 128 ? 2 : 1;  // per SM
   static constexpr int kStageKv = BITS == 4 ? kChunk / 16 * Block4<D>::kBytes : 2 * kChunk * D * 2;
   static constexpr int kBoxW = D >= 64 ? 64 : 32;                // elements per box
   static constexpr int kBlocks = D / kBoxW;
@@ -72,17 +72,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -112,10 +112,13 @@ struct Seen {
     const int back = newest - (r - sp);
     return r < live && (r < sp ? r < sinks : (back < 0 ? back + ring : back) < limit);
   }
-  // rows [r, r + 16) (r a multiple of 16) as a bit mask; one lane per row where they are not plainly all seen
-  __device__ __forceinline__ unsigned group(int r, int lane) const {
+  // are rows [r, r + n) plainly all seen?
+  __device__ __forceinline__ bool whole(int r, int n) const {
     const int first = r - sp, back = newest - first;  // of the first row
-    if (first >= 0 && r + 16 <= live && (limit == ring || (back >= 15 && back < limit))) return 0xffffu;
+    return first >= 0 && r + n <= live && (limit == ring || (back >= n - 1 && back < limit));
+  }
+  // rows [r, r + 16) (r a multiple of 16) as a bit mask, one lane per row
+  __device__ __forceinline__ unsigned group(int r, int lane) const {
     return __ballot_sync(0xffffffffu, visible(r + (lane & 15))) & 0xffffu;
   }
 };
@@ -251,8 +254,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
     tc::fence_barrier_init();
     *abort_flag = 0;
   }
-  pdl_trigger();  // (the join kernel may be staged; it waits for this grid)
   pdl_wait();
+  pdl_trigger();  // (the join kernel may be staged; it waits for this grid)
   build_prefix(W, lens, with_new ? 1 : 0, CH, b0, nb, pre, tid, GM::kThreads);  // (with a new token lens are its positions)
   const int total_f = pre[nb] * Hkv;
 
@@ -424,21 +427,25 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
       }
 
       // ---- this warp's rows: groups of 16, kMathWarps * 16 apart
-      const int row0 = (pl.c + j) * CH + warp * 16;
-      unsigned vis[NT], any = 0, all = 0xffffu;
+      const int chunk0 = (pl.c + j) * CH, row0 = chunk0 + warp * 16;
+      const bool has_new = with_new && (unsigned)(new_row - chunk0) < (unsigned)CH;
+      unsigned vis[NT], any = ok ? 0xffffu : 0u, all = 0xffffu;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        vis[u] = seen.group(row0 + u * (kMathWarps * 16), lane);
-        any |= vis[u];
-        all &= vis[u];
-      }
+      for (int u = 0; u < NT; ++u) vis[u] = 0xffffu;
       bool patched = false;
-      if (any && ok) {
+      if (ok && (has_new || !seen.whole(chunk0, CH))) {
+        any = 0;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          vis[u] = seen.group(row0 + u * (kMathWarps * 16), lane);
+          any |= vis[u];
+          all &= vis[u];
+        }
         // the new token's row: into the stage (what was loaded there is stale) and into memory
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
           const int r = row0 + u * (kMathWarps * 16);
-          if (with_new && (new_row >> 4) == (r >> 4)) {
+          if (has_new && (new_row >> 4) == (r >> 4)) {
             patched = true;
             const size_t kvrow = (size_t)(b0 + pl.b) * Hkv + pl.h;
             const bf16* kn = k_new.row(b0 + pl.b, pl.h, 0);
@@ -449,7 +456,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             } else {
               for (int e = lane; e < D / 4; e += 32) {  // 16-byte pieces of K, then of V
                 const bool value = e >= D / 8;
-                const int c = value ? e - D / 8 : e, rr = new_row - (pl.c + j) * CH;
+                const int c = value ? e - D / 8 : e, rr = new_row - chunk0;
                 const uint4 x = *reinterpret_cast<const uint4*>((value ? vn : kn) + c * 8);
                 unsigned char* base = st + (value ? CH * D * 2 : 0);
                 if (D >= 64) base += (c >> 3) * (CH * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
@@ -461,7 +468,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             __syncwarp();
           }
         }
-        if (BITS == 4 && all != 0xffffu) {  // rows that are not to be seen: scale 0 and code 0, they add nothing
+        if (BITS == 4 && any && all != 0xffffu) {  // rows that are not to be seen: scale 0, they add nothing
           patched = true;
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
@@ -476,8 +483,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
           __syncwarp();
         }
-
-        bool raise = false;
+      }
+      if (any) {
         float r_alpha = 1.f;
         if (BITS == 4) {  // the value scales relative to R as f16, each lane a pair of rows' of a group
           uint32_t x[NT];
@@ -493,7 +500,6 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           if (top > r_bits + (6u << 7) || (r_bits == 0 && top)) {  // a scale is below 2^7 R, a weight at most 2^8: f16 holds the product
             r_alpha = r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
             r_bits = top;
-            raise = true;
           }
           const float inv = __uint_as_float((254u - (r_bits >> 7)) << 23);
 #pragma unroll
@@ -569,10 +575,6 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
-#pragma unroll
-          for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[u][hb][e] *= qs[hb][e & 1];
           if (all != 0xffffu) {
 #pragma unroll
             for (int u = 0; u < NT; ++u)
@@ -586,26 +588,22 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             if (NT == 2) x = fmaxf(x, fmaxf(sc[NT - 1][hb][e], sc[NT - 1][hb][e + 2]));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(kAll, x, 16));
+            x = fmaxf(x, __shfl_xor_sync(kAll, x, 16)) * qs[hb][e];  // (positive)
             const bool up = x > m[hb][e] + 8.f;
             alpha[hb][e] = up ? ex2(m[hb][e] - x) : 1.f;
             m[hb][e] = up ? x : m[hb][e];
-            raise |= up;
           }
         }
-        if (__any_sync(kAll, raise)) {
+        // (always: the FMA pipe is idle, and without a branch the rest of the chunk mixes with it)
 #pragma unroll
-          for (int hb = 0; hb < NH; ++hb) {
-            l[hb][0] *= alpha[hb][0];
-            l[hb][1] *= alpha[hb][1];
-            const float a0 = alpha[hb][0] * r_alpha, a1 = alpha[hb][1] * r_alpha;
+        for (int hb = 0; hb < NH; ++hb) {
+          l[hb][0] *= alpha[hb][0];
+          l[hb][1] *= alpha[hb][1];
+          const float2 a = make_float2(alpha[hb][0] * r_alpha, alpha[hb][1] * r_alpha);
 #pragma unroll
-            for (int e = 0; e < D / 16; ++e) {
-              o[hb][e][0] *= a0;
-              o[hb][e][1] *= a1;
-              o[hb][e][2] *= a0;
-              o[hb][e][3] *= a1;
-            }
+          for (int e = 0; e < D / 16; ++e) {
+            const float2 x = __fmul2_rn(make_float2(o[hb][e][0], o[hb][e][1]), a), y = __fmul2_rn(make_float2(o[hb][e][2], o[hb][e][3]), a);
+            o[hb][e][0] = x.x; o[hb][e][1] = x.y; o[hb][e][2] = y.x; o[hb][e][3] = y.y;
           }
         }
         uint32_t pb[NT][NH][2];  // weights as B fragments: rows (2t, 2t + 1), (2t + 8, 2t + 9) of head g
@@ -615,7 +613,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           for (int hb = 0; hb < NH; ++hb) {
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = ex2(sc[u][hb][e] - m[hb][e & 1]);
+            for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(sc[u][hb][e], qs[hb][e & 1], -m[hb][e & 1]));
             l[hb][0] += p[0] + p[2];
             l[hb][1] += p[1] + p[3];
             pb[u][hb][0] = movmatrix_trans(BITS == 4 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));
@@ -757,39 +755,81 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
   if (!ok) __nanosleep(1000000);  // copies in flight
 }
 
-// Joins the partial results of the kv rows that range boundaries cut: block i the row that holds boundary i + 1, if that is
-// the row's first.
+// Joins the partial results of a kv row that range boundaries cut, one block per (row, query head): block x is kv row x of the
+// launch, or, where there are more kv rows than boundaries, the row that boundary x + 1 cuts first.  The weights of all
+// partial results first (one load latency), then their weighted sum with independent loads.
 template <int D>
 __global__ void __launch_bounds__(256)
-kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, int b0, int nb, int grid, const float* __restrict__ partial,
-                       bf16* __restrict__ out) {
+kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, int b0, int nb, int grid, int by_row,
+                       const float* __restrict__ partial, bf16* __restrict__ out) {
+  constexpr int COLS = D / 2, GROUPS = 256 / COLS;  // column pairs; partial results are dealt out over GROUPS sets of threads
   extern __shared__ int pre[];
-  const int tid = threadIdx.x;
-  // (the lengths are an earlier kernel's results at the latest: with the wait ahead of them everything else is too)
-  pdl_wait();
+  __shared__ float red[2][8];
+  __shared__ float2 part[256];
+  const int tid = threadIdx.x, head = blockIdx.y;
+  // (the main kernel lets this one start once its own wait is over: the lengths may be read ahead of its end)
   build_prefix(W, lens, extra, chunk, b0, nb, pre, tid, 256);
+  float* weight = reinterpret_cast<float*>(pre + 2 * nb + 1);
   const int Hkv = W.Hkv;
   const Split sp(pre[nb] * Hkv, grid);
-  const int f = ((int)blockIdx.x + 1) * sp.per;
-  if (f >= sp.total) return;
-  const int b = find_seq(pre, nb, Hkv, f);
-  const int nc = pre[b + 1] - pre[b], rem = f - pre[b] * Hkv, h = rem / nc, row0 = f - rem % nc, row1 = row0 + nc;
-  if (row0 == f || row0 / sp.per != (int)blockIdx.x) return;  // not cut here, or another boundary's
-  const int c1 = (row1 - 1) / sp.per;
-  for (int e = tid; e < G * D / 2; e += 256) {
-    const int head = e / (D / 2), ch = (e % (D / 2)) * 2;
-    float mx = kLowest, sum = 0.f, a0 = 0.f, a1 = 0.f;
-    for (int c = blockIdx.x; c <= c1; ++c) {
-      const int slot = c == (int)blockIdx.x ? 1 : 0;  // where the row begins, and where it goes on
-      const float* src = partial + ((size_t)c * 2 + slot) * partial_floats(D, G) + (size_t)head * (D + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(src), x = *reinterpret_cast<const float2*>(src + 2 + ch);
-      const float m2 = fmaxf(mx, ml.x), f0 = ex2(mx - m2), f1 = ex2(ml.x - m2);
-      mx = m2;
-      sum = sum * f0 + ml.y * f1;
-      a0 = a0 * f0 + x.x * f1;
-      a1 = a1 * f0 + x.y * f1;
+  int b, h, row0, nc;
+  if (by_row) {
+    b = blockIdx.x / Hkv;
+    h = blockIdx.x % Hkv;
+    nc = pre[b + 1] - pre[b];
+    row0 = pre[b] * Hkv + h * nc;
+  } else {
+    const int f = ((int)blockIdx.x + 1) * sp.per;
+    if (f >= sp.total) return;
+    b = find_seq(pre, nb, Hkv, f);
+    nc = pre[b + 1] - pre[b];
+    const int rem = f - pre[b] * Hkv;
+    h = rem / nc;
+    row0 = f - rem % nc;
+    if (row0 / sp.per != (int)blockIdx.x) return;  // another boundary's
+  }
+  if (nc == 0) return;
+  const int c0 = row0 / sp.per, c1 = (row0 + nc - 1) / sp.per, n = c1 - c0 + 1;  // CTAs that hold parts of the row
+  if (n < 2) return;
+  pdl_wait();
+  // the row begins in CTA c0 (its second partial result) and goes on in the others (their first)
+  auto src = [&](int i) { return partial + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * partial_floats(D, G) + (size_t)head * (D + 2); };
+  float mx = kLowest;
+  for (int i = tid; i < n; i += 256) mx = fmaxf(mx, src(i)[0]);
+  mx = warp_max(mx);
+  if ((tid & 31) == 0) red[0][tid >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, red[0][w]);
+  float sum = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float2 ml = *reinterpret_cast<const float2*>(src(i));
+    const float f = ex2(ml.x - mx);
+    weight[i] = f;
+    sum = fmaf(f, ml.y, sum);
+  }
+  sum = warp_sum(sum);
+  if ((tid & 31) == 0) red[1][tid >> 5] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += red[1][w];
+  const int col = tid % COLS, grp = tid / COLS;
+  float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+  for (int i = grp; i < n; i += GROUPS) {
+    const float2 x = *reinterpret_cast<const float2*>(src(i) + 2 + col * 2);
+    acc.x = fmaf(weight[i], x.x, acc.x);
+    acc.y = fmaf(weight[i], x.y, acc.y);
+  }
+  part[tid] = acc;
+  __syncthreads();
+  if (grp == 0) {
+    for (int i = 1; i < GROUPS; ++i) {
+      acc.x += part[i * COLS + col].x;
+      acc.y += part[i * COLS + col].y;
     }
-    *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + b) * Hkv * G + h * G + head) * D + ch) = pack_bf16(a0 / sum, a1 / sum);
+    *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + b) * Hkv * G + h * G + head) * D + col * 2) = pack_bf16(acc.x / sum, acc.y / sum);
   }
 }
 
@@ -854,8 +894,9 @@ struct TokLaunch {
                      lens, b0, nb, stages, whole ? 1 : 0, scale * kLog2e, partial, out, status, maps);
       if (e != cudaSuccess) return e;
       if (!whole && grid > 1) {
-        e = launch_pdl(kvm_window_join_kernel<D>, dim3(grid - 1), dim3(256), (2 * nb + 1) * 4, stream, true, W, G, lens, k_new.ptr ? 1 : 0,
-                       GM::kChunk, b0, nb, grid, (const float*)partial, out);
+        const bool by_row = rows < grid;
+        e = launch_pdl(kvm_window_join_kernel<D>, dim3(by_row ? (int)rows : grid - 1, G), dim3(256), (2 * nb + 1 + grid) * 4, stream, true, W,
+                       G, lens, k_new.ptr ? 1 : 0, GM::kChunk, b0, nb, grid, by_row ? 1 : 0, (const float*)partial, out);
         if (e != cudaSuccess) return e;
       }
     }
