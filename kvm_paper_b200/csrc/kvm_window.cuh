@@ -65,7 +65,7 @@ struct Block4 {
 // the products below).
 __device__ __forceinline__ unsigned short group_scale(unsigned amax_bits, float& inv) {
   inv = 0.f;
-  if (amax_bits >= 0x7f80u) return 0x7fffu;  // infinity or NaN
+  if (amax_bits >= 0x7f80u) return 0xffffu;  // infinity or NaN (as a 16-bit integer below every scale: a maximum of scales passes it by)
   const float s = __fdiv_rn(__uint_as_float(amax_bits << 16), 6.0f);
   unsigned u = __float_as_uint(s);
   u = (u + 0x1ffffu + ((u >> 18) & 1u)) & ~0x3ffffu;

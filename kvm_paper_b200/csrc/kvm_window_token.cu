@@ -32,29 +32,36 @@ constexpr int kSmemPerSm = 228 * 1024;        // of which every CTA takes 1 KB m
 constexpr int kMaxBatch = 1024;               // sequences per launch
 constexpr float kLowest = -3e38f;             // running maximum before the first score
 
-// How a variant works.  4 bits: bound by the math warps (conversions and fixed latencies): two groups of 16 rows per warp
-// and chunk side by side, two CTAs per SM where the registers allow it, the copies (one per chunk) issued by math warp 0.
+// How a variant works.  4 bits: bound by the math warps (conversions and fixed latencies), which is why a warp takes T = 4 groups of
+// 16 rows of a chunk side by side; head dimensions below 128 leave the registers for two CTAs per SM.  Short caches of 128
+// channels are bound by the changes from kv row to kv row, which two CTAs with smaller chunks (T = 2) overlap: 64 x 8 kv
+// rows of 516 tokens 19.9 us against 26.6, 8 x 16 of 4096 25.9 against 23.2 (see kShortRows).  The copies, one per chunk, are
+// issued by math warp 0.
 // 16 bits: bound by memory: one CTA with deep stages and a producer warp of its own (many copies per chunk).
-template <int D, int BITS, int NH>
+template <int D_, int BITS_, int NH_, int T_>
 struct TokGeom {
-  static constexpr int kTiles = BITS == 4 ? 2 : 1;               // groups of 16 rows per warp and chunk
+  static constexpr int D = D_, BITS = BITS_, NH = NH_;           // NH: blocks of 8 query heads per kv head
+  static constexpr int kTiles = T_;                              // groups of 16 rows per warp and chunk
   static constexpr int kChunk = kMathWarps * 16 * kTiles;        // rows per chunk
   static constexpr bool kProducer = BITS == 16;
   static constexpr int kThreads = (kMathWarps + (kProducer ? 1 : 0)) * 32;
-  static constexpr int kCtas = BITS == 4 && D * NH <= 128 ? 2 : 1;  // per SM
+  static constexpr int kCtas = BITS == 4 && (D * NH < 128 || (D == 128 && NH == 1 && T_ == 2)) ? 2 : 1;  // per SM
   static constexpr int kStageKv = BITS == 4 ? kChunk / 16 * Block4<D>::kBytes : 2 * kChunk * D * 2;
   static constexpr int kBoxW = D >= 64 ? 64 : 32;                // elements per box
   static constexpr int kBlocks = D / kBoxW;
 };
+constexpr int kShortRows = 1536;  // cache rows per kv row up to which the variant for short caches runs
 
 struct TokSmem {
   int stage_bytes, q, ored, vscale, wred, bars, pre, total;
-  __host__ __device__ TokSmem(int kv_bytes, int D, int G, int nb, int stages) {
-    q = kv_bytes;                                            // [G][D] bf16 behind the stage's rows
+  template <typename GM>
+  __host__ __device__ TokSmem(GM, int G, int nb, int stages) {
+    constexpr int D = GM::D;
+    q = GM::kStageKv;                                          // [G][D] bf16 behind the stage's rows
     stage_bytes = (q + G * D * 2 + 1023) & ~1023;            // (boxes in the 128-byte swizzle start on 1024 bytes)
     int off = stages * stage_bytes;
     ored = off; off += kMathWarps * G * D * 4;
-    vscale = off; off += kMathWarps * 2 * 128;               // a warp's value scales as f16
+    vscale = off; off += kMathWarps * GM::kTiles * D;              // a warp's value scales as f16
     wred = off; off += 2 * kMathWarps * 16 * 4;
     bars = off; off += 2 * kMaxStages * 8 + 16;              // full, empty, abort flag
     pre = off;  off += (2 * nb + 1) * 4;
@@ -112,10 +119,11 @@ struct Seen {
     const int back = newest - (r - sp);
     return r < live && (r < sp ? r < sinks : (back < 0 ? back + ring : back) < limit);
   }
-  // are rows [r, r + n) plainly all seen?
-  __device__ __forceinline__ bool whole(int r, int n) const {
-    const int first = r - sp, back = newest - first;  // of the first row
-    return first >= 0 && r + n <= live && (limit == ring || (back >= n - 1 && back < limit));
+  // chunks [from, to) of n rows are seen whole
+  __device__ __forceinline__ void whole_chunks(int n, int& from, int& to) const {
+    const int lo = limit == ring ? sp : max(sp, sp + newest - limit + 1);  // (of a ring that has wrapped around, those below the newest row)
+    from = (lo + n - 1) / n;
+    to = (limit == ring ? live : min(live, sp + newest + 1)) / n;
   }
   // rows [r, r + 16) (r a multiple of 16) as a bit mask, one lane per row
   __device__ __forceinline__ unsigned group(int r, int lane) const {
@@ -227,16 +235,15 @@ __device__ __forceinline__ void patch4(unsigned char* sb, unsigned char* gb, con
 
 }  // namespace
 
-template <int D, int BITS, int NH>
-__global__ void __launch_bounds__(TokGeom<D, BITS, NH>::kThreads, TokGeom<D, BITS, NH>::kCtas)
+template <typename GM>
+__global__ void __launch_bounds__(GM::kThreads, GM::kCtas)
 kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens, int b0, int nb, int stages,
                         int whole_rows, float scale_log2, float* __restrict__ partial, bf16* __restrict__ out, int* __restrict__ status,
                         const __grid_constant__ TokMaps maps) {
-  using GM = TokGeom<D, BITS, NH>;
-  constexpr int NG = D / 32, NT = GM::kTiles, CH = GM::kChunk;
+  constexpr int D = GM::D, BITS = GM::BITS, NH = GM::NH, NG = D / 32, NT = GM::kTiles, CH = GM::kChunk;
   constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(1024) unsigned char smem[];
-  const TokSmem lay(GM::kStageKv, D, G, nb, stages);
+  const TokSmem lay(GM{}, G, nb, stages);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + lay.bars);
   uint64_t* empty = full + kMaxStages;
   int* pre = reinterpret_cast<int*>(smem + lay.pre);
@@ -350,7 +357,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
   float* ored = reinterpret_cast<float*>(smem + lay.ored);          // [warp][G][D]
   float* wmax = reinterpret_cast<float*>(smem + lay.wred);          // [warp][16]
   float* wsum = wmax + kMathWarps * 16;
-  uint32_t* vsc = reinterpret_cast<uint32_t*>(smem + lay.vscale + warp * 256);
+  uint32_t* vsc = reinterpret_cast<uint32_t*>(smem + lay.vscale + warp * NT * D);
   bool ok = true;  // false: a wait ran out; the warp goes on without data so that it meets the others at their barriers
   int s = 0, parity = 0;             // stage of the chunk, parity of its use
   int rs = 0, rparity = 0;           // of the chunk before it
@@ -358,7 +365,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
   for (int i = 0; i < nloc;) {  // kv rows, or what of them lies in the range
     const int cnt = min(pl.n_chunks - pl.c, nloc - i), n = tokens[pl.b];
     const Seen seen(W, n);
-    const int new_row = with_new ? W.row_of(n - 1) : -1;
+    const int new_row = with_new ? W.row_of(n - 1) : -1, new_chunk = with_new ? new_row / CH : -1;
+    int plain_from, plain_to;  // chunks that are seen whole
+    seen.whole_chunks(CH, plain_from, plain_to);
     uint32_t qf[NH][D / 16][2];      // queries as B fragments
     float qs[NH][2];                 // softmax scale (log2) of this thread's heads 2t, 2t + 1
     float o[NH][D / 16][4];          // output: channels x heads
@@ -428,19 +437,16 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
 
       // ---- this warp's rows: groups of 16, kMathWarps * 16 apart
       const int chunk0 = (pl.c + j) * CH, row0 = chunk0 + warp * 16;
-      const bool has_new = with_new && (unsigned)(new_row - chunk0) < (unsigned)CH;
-      unsigned vis[NT], any = ok ? 0xffffu : 0u, all = 0xffffu;
-#pragma unroll
-      for (int u = 0; u < NT; ++u) vis[u] = 0xffffu;
+      const bool has_new = pl.c + j == new_chunk;
+      // which of this warp's rows are to be seen, 16 bits per group
+      constexpr unsigned long long kWhole = NT == 4 ? ~0ull : (1ull << (16 * NT)) - 1;
+      unsigned long long seen_rows = ok ? kWhole : 0;
+      auto vis = [&](int u) { return (unsigned)(seen_rows >> (16 * u)) & 0xffffu; };
       bool patched = false;
-      if (ok && (has_new || !seen.whole(chunk0, CH))) {
-        any = 0;
+      if (ok && (has_new || pl.c + j < plain_from || pl.c + j >= plain_to)) {
+        seen_rows = 0;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          vis[u] = seen.group(row0 + u * (kMathWarps * 16), lane);
-          any |= vis[u];
-          all &= vis[u];
-        }
+        for (int u = 0; u < NT; ++u) seen_rows |= (unsigned long long)seen.group(row0 + u * (kMathWarps * 16), lane) << (16 * u);
         // the new token's row: into the stage (what was loaded there is stale) and into memory
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
@@ -468,14 +474,14 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             __syncwarp();
           }
         }
-        if (BITS == 4 && any && all != 0xffffu) {  // rows that are not to be seen: scale 0, they add nothing
+        if (BITS == 4 && seen_rows && seen_rows != kWhole) {  // rows that are not to be seen: scale 0, they add nothing
           patched = true;
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
             unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
             for (int e = lane; e < 16 * NG; e += 32) {
               const int rr = e / NG, grp = e % NG;
-              if (!((vis[u] >> rr) & 1)) {
+              if (!((vis(u) >> rr) & 1)) {
                 *reinterpret_cast<unsigned short*>(sb + Block4<D>::kKeyScales + rr * (2 * NG) + grp * 2) = 0;
                 *reinterpret_cast<unsigned short*>(sb + Block4<D>::kValueScales + (rr >> 1) * (4 * NG) + grp * 4 + (rr & 1) * 2) = 0;
               }
@@ -484,38 +490,38 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           __syncwarp();
         }
       }
-      if (any) {
+      // groups u0 .. u0 + N - 1 of this warp's rows
+      auto groups = [&](auto count, int u0) {
+        constexpr int N = decltype(count)::value;
         float r_alpha = 1.f;
         if (BITS == 4) {  // the value scales relative to R as f16, each lane a pair of rows' of a group
-          uint32_t x[NT];
-          unsigned top = 0;
+          uint32_t x[N], top2 = 0;
 #pragma unroll
-          for (int u = 0; u < NT; ++u) {
-            x[u] = lane < 8 * NG ? *reinterpret_cast<const uint32_t*>(st + (warp + u * kMathWarps) * Block4<D>::kBytes + Block4<D>::kValueScales + lane * 4) : 0u;
-            // the exponent of the largest of them (NaN does not count: it reaches its own group only)
-            const unsigned x0 = x[u] & 0xffffu, x1 = x[u] >> 16;
-            top = max(top, max(x0 < 0x7f80u ? x0 : 0u, x1 < 0x7f80u ? x1 : 0u));
+          for (int u = 0; u < N; ++u) {
+            x[u] = lane < 8 * NG ? *reinterpret_cast<const uint32_t*>(st + (warp + (u0 + u) * kMathWarps) * Block4<D>::kBytes + Block4<D>::kValueScales + lane * 4) : 0u;
+            top2 = __vmaxs2(top2, x[u]);  // (the NaN of a scale is negative: it reaches its own group only)
           }
-          top = __reduce_max_sync(kAll, top) & 0x7f80u;
+          // the exponent of the largest of them
+          const unsigned top = __reduce_max_sync(kAll, max(top2 & 0xffffu, top2 >> 16)) & 0x7f80u;
           if (top > r_bits + (6u << 7) || (r_bits == 0 && top)) {  // a scale is below 2^7 R, a weight at most 2^8: f16 holds the product
             r_alpha = r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
             r_bits = top;
           }
           const float inv = __uint_as_float((254u - (r_bits >> 7)) << 23);
 #pragma unroll
-          for (int u = 0; u < NT; ++u)
-            if (lane < 8 * NG) vsc[u * 32 + lane] = pack_f16(__uint_as_float(x[u] << 16) * inv, __uint_as_float(x[u] & 0xffff0000u) * inv);
+          for (int u = 0; u < N; ++u)
+            if (lane < 8 * NG) vsc[u * 8 * NG + lane] = pack_f16(__uint_as_float(x[u] << 16) * inv, __uint_as_float(x[u] & 0xffff0000u) * inv);
           __syncwarp();
         }
 
         // ---- scores: rows g, g + 8 x heads 2t, 2t + 1
-        float sc[NT][NH][4];
+        float sc[N][NH][4];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
+        for (int u = 0; u < N; ++u) {
 #pragma unroll
           for (int hb = 0; hb < NH; ++hb) sc[u][hb][0] = sc[u][hb][1] = sc[u][hb][2] = sc[u][hb][3] = 0.f;
           if constexpr (BITS == 4) {
-            const unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
+            const unsigned char* sb = st + (warp + (u0 + u) * kMathWarps) * Block4<D>::kBytes;
             uint32_t kw[2][NG];
             float ks[2][NG];
 #pragma unroll
@@ -575,17 +581,18 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
-          if (all != 0xffffu) {
+          if (seen_rows != kWhole) {
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
+            for (int u = 0; u < N; ++u)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (!((vis[u] >> (g + (e >> 1) * 8)) & 1)) sc[u][hb][e] = -INFINITY;
+                if (!((vis(u0 + u) >> (g + (e >> 1) * 8)) & 1)) sc[u][hb][e] = -INFINITY;
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float x = fmaxf(sc[0][hb][e], sc[0][hb][e + 2]);
-            if (NT == 2) x = fmaxf(x, fmaxf(sc[NT - 1][hb][e], sc[NT - 1][hb][e + 2]));
+#pragma unroll
+            for (int u = 1; u < N; ++u) x = fmaxf(x, fmaxf(sc[u][hb][e], sc[u][hb][e + 2]));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 16)) * qs[hb][e];  // (positive)
@@ -606,9 +613,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             o[hb][e][0] = x.x; o[hb][e][1] = x.y; o[hb][e][2] = y.x; o[hb][e][3] = y.y;
           }
         }
-        uint32_t pb[NT][NH][2];  // weights as B fragments: rows (2t, 2t + 1), (2t + 8, 2t + 9) of head g
+        uint32_t pb[N][NH][2];  // weights as B fragments: rows (2t, 2t + 1), (2t + 8, 2t + 9) of head g
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int u = 0; u < N; ++u)
 #pragma unroll
           for (int hb = 0; hb < NH; ++hb) {
             float p[4];
@@ -622,12 +629,12 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
 
         // ---- output += V^T P
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
+        for (int u = 0; u < N; ++u) {
           if constexpr (BITS == 4) {
-            const unsigned char* sb = st + (warp + u * kMathWarps) * Block4<D>::kBytes;
+            const unsigned char* sb = st + (warp + (u0 + u) * kMathWarps) * Block4<D>::kBytes;
             uint32_t vs[2][NG];  // value scales of row pairs t and t + 4
-            lds(vs[0], vsc + u * 32 + t * NG);
-            lds(vs[1], vsc + u * 32 + (t + 4) * NG);
+            lds(vs[0], vsc + u * 8 * NG + t * NG);
+            lds(vs[1], vsc + u * 8 * NG + (t + 4) * NG);
             constexpr int NWD = NG > 1 ? NG / 2 : 1;  // 32-bit words of codes per thread and row
             uint32_t vw[4][NWD];
 #pragma unroll
@@ -672,7 +679,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
               for (int r = 0; r < 4; ++r) {
                 const int rr = warp * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
                 lds(x[r], D >= 64 ? vb + blk * (CH * 128) + rr * 128 + ((g ^ (rr & 7)) << 4) : vb + rr * 64 + g * 8);
-                if (all != 0xffffu && !((vis[u] >> (rr & 15)) & 1)) {  // (0 x NaN)
+                if (seen_rows != kWhole && !((vis(u0 + u) >> (rr & 15)) & 1)) {  // (0 x NaN)
 #pragma unroll
                   for (int w = 0; w < WORDS; ++w) x[r][w] = 0;
                 }
@@ -687,6 +694,12 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             }
           }
         }
+      };
+      if (seen_rows) {
+        // side by side; a single group with rows to be seen (the end of a cache) by itself
+        const int lowest = (__ffsll((long long)seen_rows) - 1) >> 4;
+        if (NT == 1 || (seen_rows >> (16 * lowest)) > 0xffffu) groups(std::integral_constant<int, NT>{}, 0);
+        else groups(std::integral_constant<int, 1>{}, lowest);
         if (patched) tc::fence_proxy_async();  // before the next copy into this stage
       }
       __syncwarp();
@@ -839,9 +852,9 @@ namespace {
 struct TokPlan {
   // sequences whose lengths fit beside two stages
   template <typename GM>
-  static int sequences(int D, int G, int limit) {
+  static int sequences(int G, int limit) {
     int n = kMaxBatch;
-    while (n > 16 && TokSmem(GM::kStageKv, D, G, n, 2).total > limit) n -= 16;
+    while (n > 16 && TokSmem(GM{}, G, n, 2).total > limit) n -= 16;
     return n;
   }
   // Whole kv rows per CTA where cutting them gains less than the second launch and the partial results cost (about 2.5 us;
@@ -855,13 +868,13 @@ struct TokPlan {
   }
 };
 
-template <int D, int BITS, int NH>
+template <typename GM>
 struct TokLaunch {
-  using GM = TokGeom<D, BITS, NH>;
+  static constexpr int D = GM::D, BITS = GM::BITS;
   static constexpr int kSmemLimit = kSmemPerSm / GM::kCtas - 1024;
 
   static size_t workspace(const WindowDev& W, int G) {
-    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(D, G, kSmemLimit);
+    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(G, kSmemLimit);
     for (int b0 = 0; b0 < W.batch; b0 += per)
       if (!TokPlan::whole_rows<GM>(W, std::min(per, W.batch - b0), ctas)) return (size_t)ctas * 2 * partial_floats(D, G) * 4;
     return 0;
@@ -877,20 +890,20 @@ struct TokLaunch {
       if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box))
         return cudaErrorInvalidValue;
     }
-    auto kern = kvm_window_token_kernel<D, BITS, NH>;
+    auto kern = kvm_window_token_kernel<GM>;
     static std::atomic<unsigned long long> raised{0};
     cudaError_t e = raise_smem_limit(kern, kSmemLimit, raised);
     if (e != cudaSuccess) return e;
-    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(D, G, kSmemLimit);
+    const int ctas = window_sm_count() * GM::kCtas, per = TokPlan::sequences<GM>(G, kSmemLimit);
     const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
     for (int b0 = 0; b0 < W.batch; b0 += per) {
       const int nb = std::min(per, W.batch - b0);
       int stages = 2;
-      while (stages < kMaxStages && TokSmem(GM::kStageKv, D, G, nb, stages + 1).total <= kSmemLimit) ++stages;
+      while (stages < kMaxStages && TokSmem(GM{}, G, nb, stages + 1).total <= kSmemLimit) ++stages;
       const bool whole = TokPlan::whole_rows<GM>(W, nb, ctas);
       const long long rows = (long long)nb * W.Hkv;
       const int grid = (int)std::min<long long>(ctas, whole ? rows : rows * max_chunks);
-      e = launch_pdl(kern, dim3(grid), dim3(GM::kThreads), TokSmem(GM::kStageKv, D, G, nb, stages).total, stream, true, W, G, q, k_new, v_new,
+      e = launch_pdl(kern, dim3(grid), dim3(GM::kThreads), TokSmem(GM{}, G, nb, stages).total, stream, true, W, G, q, k_new, v_new,
                      lens, b0, nb, stages, whole ? 1 : 0, scale * kLog2e, partial, out, status, maps);
       if (e != cudaSuccess) return e;
       if (!whole && grid > 1) {
@@ -904,28 +917,37 @@ struct TokLaunch {
   }
 };
 
+template <int D, int NH>
+struct TokTiles {  // groups per warp and chunk, 4 bits
+  static constexpr int value = D * NH == 256 ? 2 : 4;
+};
+
 template <typename F>
-auto token_variant(int D, int bits, int G, F f) {
-  auto heads = [&](auto d, auto b) {
-    constexpr int kD = decltype(d)::value, kB = decltype(b)::value;
-    return G <= 8 ? f(TokLaunch<kD, kB, 1>{}) : f(TokLaunch<kD, kB, 2>{});
+auto token_variant(int D, int bits, const WindowDev& W, int G, F f) {
+  auto heads = [&](auto d, auto h) {
+    constexpr int kD = decltype(d)::value, kH = decltype(h)::value;
+    if (bits == 16) return f(TokLaunch<TokGeom<kD, 16, kH, 1>>{});
+    if constexpr (kD == 128 && kH == 1) {
+      if (W.rows <= kShortRows) return f(TokLaunch<TokGeom<kD, 4, kH, 2>>{});
+    }
+    return f(TokLaunch<TokGeom<kD, 4, kH, TokTiles<kD, kH>::value>>{});
   };
-  auto width = [&](auto b) {
-    return D == 128 ? heads(std::integral_constant<int, 128>{}, b)
-                    : D == 64 ? heads(std::integral_constant<int, 64>{}, b) : heads(std::integral_constant<int, 32>{}, b);
+  auto width = [&](auto h) {
+    return D == 128 ? heads(std::integral_constant<int, 128>{}, h)
+                    : D == 64 ? heads(std::integral_constant<int, 64>{}, h) : heads(std::integral_constant<int, 32>{}, h);
   };
-  return bits == 4 ? width(std::integral_constant<int, 4>{}) : width(std::integral_constant<int, 16>{});
+  return G <= 8 ? width(std::integral_constant<int, 1>{}) : width(std::integral_constant<int, 2>{});
 }
 
 }  // namespace
 
 size_t window_token_workspace(int D, int bits, const WindowDev& W, int G) {
-  return token_variant(D, bits, G, [&](auto v) { return v.workspace(W, G); });
+  return token_variant(D, bits, W, G, [&](auto v) { return v.workspace(W, G); });
 }
 
 cudaError_t window_token_dispatch(int D, int bits, const WindowDev& W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_new, SeqInts lens,
                                   float scale, float* partial, bf16* out, int* status, cudaStream_t stream) {
-  return token_variant(D, bits, G, [&](auto v) { return v.run(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream); });
+  return token_variant(D, bits, W, G, [&](auto v) { return v.run(W, G, q, k_new, v_new, lens, scale, partial, out, status, stream); });
 }
 
 }  // namespace kvm
