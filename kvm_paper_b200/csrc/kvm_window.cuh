@@ -61,26 +61,41 @@ struct Block4 {
   static constexpr int kGroups = D / 32;
 };
 
-// The scale of a group from the largest of its magnitudes' bf16 bit patterns (bf16 bits of the scale, and 1 / scale for
-// the products below).
+// The scale of a group from the largest of its magnitudes' bf16 bit patterns: bf16 bits, and a reciprocal for the products
+// below.  m / 6 is formed as a product and rounded to 16 significant bits first: m has 8 of them, so a quotient that is not
+// on the border between two 6-bit numbers is at least 2^-11 away from it, one that is comes out exactly.
 __device__ __forceinline__ unsigned short group_scale(unsigned amax_bits, float& inv) {
   inv = 0.f;
   if (amax_bits >= 0x7f80u) return 0xffffu;  // infinity or NaN (as a 16-bit integer below every scale: a maximum of scales passes it by)
-  const float s = __fdiv_rn(__uint_as_float(amax_bits << 16), 6.0f);
-  unsigned u = __float_as_uint(s);
+  unsigned u = __float_as_uint(__uint_as_float(amax_bits << 16) * (1.0f / 6.0f));
+  u = (u + 0x80u) & ~0xffu;
   u = (u + 0x1ffffu + ((u >> 18) & 1u)) & ~0x3ffffu;
   if (u < 0x00800000u) return 0;
-  inv = __frcp_rn(__uint_as_float(u));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__uint_as_float(u)));
   return (unsigned short)(u >> 16);
 }
 // x / s to within 2^-14, exact where it lies on the border between two levels: x has 8 and s 6 significant bits, so a
-// quotient off the border is at least 2^-9 away from it, and the product with the rounded reciprocal errs by less than 2^-20.
-__device__ __forceinline__ float level_of(float x, float inv) { return __fadd_rn(__fadd_rn(__fmul_rn(x, inv), 768.f), -768.f); }
+// quotient off the border is at least 2^-9 away from it, and the product with the reciprocal errs by less than 2^-19.
+__device__ __forceinline__ float2 levels_of(unsigned x2, float inv) {
+  const float2 r = __fmul2_rn(unpack_bf16(x2), make_float2(inv, inv));
+  return __fadd2_rn(__fadd2_rn(r, make_float2(768.f, 768.f)), make_float2(-768.f, -768.f));
+}
 
-// two levels -> one byte of e2m1 codes (lo in the low nibble), nearest, ties to even, saturating
-__device__ __forceinline__ unsigned e2m1x2(float lo, float hi) {
+// levels -> e2m1 codes (the first in the lowest nibble), nearest, ties to even, saturating
+__device__ __forceinline__ unsigned e2m1x4(float2 a, float2 b) {
   unsigned r;
-  asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+  asm("{\n\t.reg .b8 x, y, z;\n\tcvt.rn.satfinite.e2m1x2.f32 x, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 y, %4, %3;\n\tcvt.u8.u32 z, 0;\n\t"
+      "mov.b32 %0, {x, y, z, z};\n\t}"
+      : "=r"(r)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ unsigned e2m1x8(float2 a, float2 b, float2 c, float2 d) {
+  unsigned r;
+  asm("{\n\t.reg .b8 x, y, z, w;\n\tcvt.rn.satfinite.e2m1x2.f32 x, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 y, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 z, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 w, %8, %7;\n\tmov.b32 %0, {x, y, z, w};\n\t}"
+      : "=r"(r)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y), "f"(d.x), "f"(d.y));
   return r;
 }
 // 8 codes -> 4 x f16x2 (byte i of the word -> o[i], low nibble in the low half)

@@ -1,5 +1,7 @@
 // Writing tokens into a window cache (in 4 bits: quantised on the way) and reading back what it holds, in order.
 // Both are one pass over memory.
+#include <algorithm>
+
 #include "kvm_window.cuh"
 
 namespace kvm {
@@ -7,6 +9,7 @@ namespace kvm {
 namespace {
 
 constexpr int kStoreThreads = 256;
+constexpr int kRowsPerZ = 32768;  // kv rows along y of the grid, the rest along z
 constexpr int kStoreUnroll = 4;  // rows in flight per thread
 
 __device__ __forceinline__ unsigned abs_max_bits(const uint4& x) {
@@ -15,6 +18,12 @@ __device__ __forceinline__ unsigned abs_max_bits(const uint4& x) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
   return max(m & 0xffffu, m >> 16);
+}
+
+// ring place of the token that is `i`-th behind the sinks (before them: where it would be), once per thread
+__device__ __forceinline__ int ring_place(int i, int ring) {
+  const int r = i % ring;
+  return r < 0 ? r + ring : r;
 }
 
 }  // namespace
@@ -29,13 +38,7 @@ __device__ __forceinline__ void store_row4(unsigned char* block, int rr, int c, 
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   float inv;
   const unsigned short s = group_scale(m, inv);
-  const unsigned w[4] = {x.x, x.y, x.z, x.w};
-  unsigned code = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack_bf16(w[i]);
-    code |= e2m1x2(level_of(f.x, inv), level_of(f.y, inv)) << (8 * i);
-  }
+  unsigned code = e2m1x8(levels_of(x.x, inv), levels_of(x.y, inv), levels_of(x.z, inv), levels_of(x.w, inv));
   if (m >= 0x7f80u) code = 0;
   const int n = c >> 2, u = c & 3;  // group, eighth channels inside it
   if (value) {
@@ -60,12 +63,14 @@ __device__ __forceinline__ void store_row4(unsigned char* block, int rr, int c, 
 // are still in it behind the last one (no two tokens of a call share a row).
 template <int D, int BITS>
 __global__ void __launch_bounds__(kStoreThreads)
-kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, int tiles, SeqInts positions,
+kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, SeqInts positions,
                         SeqInts lengths) {
   constexpr int TPR = D / 8;                          // threads per row
   constexpr int RPI = kStoreThreads / TPR / 2;        // rows per iteration (keys and values side by side)
   pdl_wait();
-  const int kvrow = blockIdx.x / tiles, b = kvrow / W.Hkv, h = kvrow % W.Hkv;
+  const int kvrow = blockIdx.z * kRowsPerZ + blockIdx.y;
+  if (kvrow >= W.batch * W.Hkv) return;
+  const int b = kvrow / W.Hkv, h = kvrow % W.Hkv;
   const int pos = positions.at(b), len = min(lengths.at(b), n_tokens);
   if (pos < 0 || len <= 0) return;
   const int tid = threadIdx.x, c = tid % TPR, vr = tid / TPR;
@@ -73,7 +78,7 @@ kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, int til
   const int r0 = vr - (value ? RPI : 0);
   const Tensor4& src = value ? v : k;
   const long long end = (long long)pos + len, first = end - W.ring;  // tokens from `first` on stay in the ring
-  const int base = (int)(blockIdx.x % tiles) * (RPI * kStoreUnroll);
+  const int base = (int)blockIdx.x * (RPI * kStoreUnroll);
   if (base >= len || ((long long)pos + base >= W.sinks && (long long)pos + base + RPI * kStoreUnroll <= first)) return;
   uint4 x[kStoreUnroll];
 #pragma unroll
@@ -81,12 +86,15 @@ kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, int til
     const int tok = base + i * RPI + r0;
     x[i] = tok < len ? *reinterpret_cast<const uint4*>(src.row(b, h, tok) + c * 8) : make_uint4(0, 0, 0, 0);
   }
+  const int ring0 = ring_place(pos + base - W.sinks, W.ring);
 #pragma unroll
   for (int i = 0; i < kStoreUnroll; ++i) {
     const int tok = base + i * RPI + r0;
     const long long p = (long long)pos + tok;
     const bool write = tok < len && (p < W.sinks || p >= first);
-    const int r = write ? W.row_of((int)p) : 0;
+    int r = ring0 + i * RPI + r0;
+    if (r >= W.ring) r = W.ring >= RPI * kStoreUnroll ? r - W.ring : r % W.ring;
+    r = !write ? 0 : (p < W.sinks ? (int)p : W.sp + r);
     if (BITS == 16) {
       if (write) *reinterpret_cast<uint4*>((value ? W.v : W.k) + ((size_t)kvrow * W.rows + r) * D + c * 8) = x[i];
     } else {
@@ -98,25 +106,31 @@ kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, int til
 // Rows i < min(n, sinks + window) of the output: the first sinks tokens, then the last `window`; zeros behind them.
 template <int D, int BITS>
 __global__ void __launch_bounds__(kStoreThreads)
-kvm_window_read_kernel(WindowDev W, int tiles, SeqInts lengths, bf16* __restrict__ k_out, bf16* __restrict__ v_out) {
+kvm_window_read_kernel(WindowDev W, SeqInts lengths, bf16* __restrict__ k_out, bf16* __restrict__ v_out) {
   constexpr int TPR = D / 8;
   constexpr int RPI = kStoreThreads / TPR / 2;
   constexpr int NG = Block4<D>::kGroups;
   pdl_wait();
   const int keep = W.sinks + W.window;
-  const int kvrow = blockIdx.x / tiles, b = kvrow / W.Hkv;
+  const int kvrow = blockIdx.z * kRowsPerZ + blockIdx.y;
+  if (kvrow >= W.batch * W.Hkv) return;
+  const int b = kvrow / W.Hkv;
   const int n = max(lengths.at(b), 0), held = min(n, keep);
   const int tid = threadIdx.x, c = tid % TPR, vr = tid / TPR;
   const bool value = vr >= RPI;
   const int r0 = vr - (value ? RPI : 0);
-  const int base = (int)(blockIdx.x % tiles) * (RPI * kStoreUnroll);
+  const int base = (int)blockIdx.x * (RPI * kStoreUnroll);
+  if (base >= keep) return;
+  const int ring0 = ring_place(n - held + base - W.sinks, W.ring);
   uint4 x[kStoreUnroll];
 #pragma unroll
   for (int i = 0; i < kStoreUnroll; ++i) {
     const int at = base + i * RPI + r0;
     x[i] = make_uint4(0, 0, 0, 0);
     if (at >= held) continue;
-    const int r = W.row_of(at < W.sinks ? at : n - held + at);
+    int r = ring0 + i * RPI + r0;
+    if (r >= W.ring) r = W.ring >= RPI * kStoreUnroll ? r - W.ring : r % W.ring;
+    r = at < W.sinks ? at : W.sp + r;
     if (BITS == 16) {
       x[i] = *reinterpret_cast<const uint4*>((value ? W.v : W.k) + ((size_t)kvrow * W.rows + r) * D + c * 8);
     } else {
@@ -149,7 +163,8 @@ kvm_window_read_kernel(WindowDev W, int tiles, SeqInts lengths, bf16* __restrict
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
-        z[j] = pack_bf16(f.x * s, f.y * s);  // exact
+        const float2 y2 = __fmul2_rn(f, make_float2(s, s));  // exact
+        z[j] = pack_bf16(y2.x, y2.y);
       }
       y = make_uint4(z[0], z[1], z[2], z[3]);
     }
@@ -159,21 +174,23 @@ kvm_window_read_kernel(WindowDev W, int tiles, SeqInts lengths, bf16* __restrict
 
 namespace {
 
+// tiles x kv rows
+bool store_grid(const WindowDev& W, int n, int rows, dim3& grid) {
+  const long long kvrows = (long long)W.batch * W.Hkv, z = (kvrows + kRowsPerZ - 1) / kRowsPerZ;
+  grid = dim3((n + rows - 1) / rows, (unsigned)std::min<long long>(kvrows, kRowsPerZ), (unsigned)z);
+  return z < 65536;
+}
 template <int D, int BITS>
 cudaError_t launch_write(const WindowDev& W, Tensor4 k, Tensor4 v, int n_tokens, SeqInts positions, SeqInts lengths, cudaStream_t stream) {
-  constexpr int rows = kStoreThreads / (D / 8) / 2 * kStoreUnroll;
-  const int tiles = (n_tokens + rows - 1) / rows;
-  if ((long long)tiles * W.batch * W.Hkv > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(kvm_window_write_kernel<D, BITS>, dim3(tiles * W.batch * W.Hkv), dim3(kStoreThreads), 0, stream, true, W, k, v,
-                    n_tokens, tiles, positions, lengths);
+  dim3 grid;
+  if (!store_grid(W, n_tokens, kStoreThreads / (D / 8) / 2 * kStoreUnroll, grid)) return cudaErrorInvalidValue;
+  return launch_pdl(kvm_window_write_kernel<D, BITS>, grid, dim3(kStoreThreads), 0, stream, true, W, k, v, n_tokens, positions, lengths);
 }
 template <int D, int BITS>
 cudaError_t launch_read(const WindowDev& W, SeqInts lengths, bf16* k_out, bf16* v_out, cudaStream_t stream) {
-  constexpr int rows = kStoreThreads / (D / 8) / 2 * kStoreUnroll;
-  const int tiles = (W.sinks + W.window + rows - 1) / rows;
-  if ((long long)tiles * W.batch * W.Hkv > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(kvm_window_read_kernel<D, BITS>, dim3(tiles * W.batch * W.Hkv), dim3(kStoreThreads), 0, stream, true, W, tiles, lengths,
-                    k_out, v_out);
+  dim3 grid;
+  if (!store_grid(W, W.sinks + W.window, kStoreThreads / (D / 8) / 2 * kStoreUnroll, grid)) return cudaErrorInvalidValue;
+  return launch_pdl(kvm_window_read_kernel<D, BITS>, grid, dim3(kStoreThreads), 0, stream, true, W, lengths, k_out, v_out);
 }
 
 }  // namespace

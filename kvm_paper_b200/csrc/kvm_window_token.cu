@@ -214,8 +214,7 @@ __device__ __forceinline__ void patch4(unsigned char* sb, unsigned char* gb, con
     for (int d = 1; d < 8; d <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, d));  // 8 lanes hold a group
     float inv;
     const unsigned short sc = group_scale(am, inv);
-    const float2 f0 = unpack_bf16(x.x), f1 = unpack_bf16(x.y);
-    unsigned code = e2m1x2(level_of(f0.x, inv), level_of(f0.y, inv)) | e2m1x2(level_of(f1.x, inv), level_of(f1.y, inv)) << 8;
+    unsigned code = e2m1x4(levels_of(x.x, inv), levels_of(x.y, inv));
     if (am >= 0x7f80u) code = 0;
     const int grp = c4 >> 3, u = c4 & 7;
     const int off = value ? Block4<D>::kValues + rr * (D / 2) + u * (2 * NG) + grp * 2
