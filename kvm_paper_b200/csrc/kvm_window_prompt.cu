@@ -31,6 +31,7 @@ constexpr int kRows = 128;   // queries per tile, keys per tile
 constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kMaxListed = 500;   // sequences of a batch of unequal lengths whose tiles are listed
 constexpr int kSplit = 3;         // of 4 x 32 keys, those whose weights are handed to the MMA warp first
 constexpr int kPoly = 4;          // of 16 pairs of weights, those formed by polynomial
 constexpr int kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
@@ -43,7 +44,8 @@ struct PC {
   static constexpr int kSlots = DP == 128 ? 5 : 8;
   static constexpr int kOffKv = 2 * kTileBytes;
   static constexpr int kOffBar = kOffKv + kSlots * kTileBytes;
-  static constexpr int kSmem = kOffBar + 512;
+  static constexpr int kOffPre = kOffBar + 512;
+  static constexpr int kSmem = kOffPre + (kMaxListed + 1) * 4;
   static constexpr uint32_t kColO = 256;  // first column of the outputs; scores of tile i in columns 128 i ..
 };
 
@@ -63,15 +65,30 @@ struct PromptArgs {
   int q_head_inner, k_head_inner, v_head_inner;
 };
 
-// What an item is, computed alike by every role.
+// What an item is, computed alike by every role.  LISTED: batches of unequal lengths, whose items are the tiles that exist, found
+// through a prefix over the sequences (a template: the few registers cost the others 2 %).
+template <bool LISTED>
 struct Item {
   int b, hkv, len, lo, s_end, n_sink, n_tiles;  // first window key, end of the sinks before it, their tiles, tiles in all
   int hq[2], t0[2], begin[2], end[2];           // per query tile: head, first query, window tiles [begin, end) in list places
-  __device__ __forceinline__ Item(const PromptArgs& a, int x) {
-    const int qt = a.q_tiles - 1 - x / a.units, u = x % a.units;  // (later, heavier tiles first)
+  __device__ __forceinline__ Item(const PromptArgs& a, const int* pre, int x) {
     const int per_seq = a.units / a.B, G = a.Hq / a.Hkv;
-    b = u / per_seq;
-    const int hu = u % per_seq;
+    int qt, hu;
+    if (LISTED) {  // sequence by sequence, later tiles first
+      const int t = x / per_seq;
+      int lo_b = 0, hi_b = a.B - 1;  // last b with pre[b] <= t: one that has tiles
+      while (lo_b < hi_b) {
+        const int mid = (lo_b + hi_b + 1) >> 1;
+        if (pre[mid] <= t) lo_b = mid; else hi_b = mid - 1;
+      }
+      b = lo_b;
+      qt = pre[b + 1] - 1 - t;
+      hu = x % per_seq;
+    } else {  // later, heavier tiles of all sequences first
+      qt = a.q_tiles - 1 - x / a.units;
+      b = (x % a.units) / per_seq;
+      hu = x % per_seq;
+    }
     if (a.pair_heads) {
       hq[0] = hu * 2;
       hq[1] = hq[0] + 1;
@@ -165,18 +182,18 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
 }
 
 // ------------------------------------------------------------------------------------------ producer
-template <int DP>
-__device__ __forceinline__ bool produce(const PromptArgs& a, unsigned char* smem, PromptBars* bars) {
+template <int DP, bool LISTED>
+__device__ __forceinline__ bool produce(const PromptArgs& a, const int* pre, int n_items, unsigned char* smem, PromptBars* bars) {
   int slot = 0, round = 0;  // of the ring
-  auto kv = [&](const CUtensorMap* m, bool hi, int key, const Item& it) {
+  auto kv = [&](const CUtensorMap* m, bool hi, int key, const Item<LISTED>& it) {
     if (round > 0 && !wait(&bars->kv_empty[slot], (round - 1) & 1)) return false;
     load_tile<DP>(smem + PC<DP>::kOffKv + slot * PC<DP>::kTileBytes, m, hi, key, it.hkv, it.b, &bars->kv_full[slot]);
     if (++slot == PC<DP>::kSlots) { slot = 0; ++round; }
     return true;
   };
   int nq[2] = {0, 0};
-  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
-    const Item it(a, x);
+  for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
+    const Item<LISTED> it(a, pre, x);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (it.end[i] == 0) continue;
@@ -262,8 +279,8 @@ struct Issuer {
   }
 };
 
-template <int DP>
-__device__ __forceinline__ bool issue(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem) {
+template <int DP, bool LISTED>
+__device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n_items, unsigned char* smem, PromptBars* bars, uint32_t tmem) {
   Issuer<DP> is;
   is.bars = bars;
   is.tmem = tmem;
@@ -271,8 +288,8 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, unsigned char* smem, 
   is.dk = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
   is.dv = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);
   int slot = 0, round = 0;
-  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
-    const Item it(a, x);
+  for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
+    const Item<LISTED> it(a, pre, x);
     const int cnt0 = it.count(0), cnt1 = it.count(1);
     int done0 = 0, done1 = 0;
     for (int u = 0; u < it.n_tiles; ++u) {
@@ -345,14 +362,15 @@ __device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hk
   }
 }
 
-template <int DP>
-__device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem, PromptBars* bars, uint32_t tmem, int I, int row, int wq, int lane) {
+template <int DP, bool LISTED>
+__device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int n_items, unsigned char* smem, PromptBars* bars, uint32_t tmem,
+                                        int I, int row, int wq, int lane) {
   const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
   const uint32_t col_s = lane_addr + I * 128, col_o = lane_addr + PC<DP>::kColO + I * DP;
   const float sc = a.scale_log2;
   int slot = 0, round = 0, n = 0, ni = 0;
-  for (int x = blockIdx.x; x < a.n_items; x += gridDim.x) {
-    const Item it(a, x);
+  for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
+    const Item<LISTED> it(a, pre, x);
     const int t = it.pick(it.t0, I) + row, p0 = a.S - a.T + it.pick(it.t0, I), p = p0 + row;
     float m_run = -INFINITY, l_run = 0.f;
     bool poison = false;
@@ -414,9 +432,6 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
         l_run *= alpha;
         m_run = m_new;
       }
-      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
-      float2 ls = make_float2(0.f, 0.f);
       // value rows behind the sequence's length: padding, cleared before the product reads them
       if (it.len < a.S && key0 + kRows > it.len) {
         if (!warp_wait(&bars->kv_full[vs], vr)) return false;
@@ -429,17 +444,19 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
       }
       // weights; where every key is seen, some by polynomial (a masked weight has to be 0, which the polynomial's range
       // does not hold)
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
       const float sc128 = sc * (1.f / 128.f), nm128 = (neg_m + 120.f) * (1.f / 128.f);
+      float2 ls = make_float2(0.f, 0.f);
       auto weights = [&](auto poly) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int part = 0; part < 2; ++part) {
 #pragma unroll
-          for (int c = half * kSplit; c < (half ? 4 : kSplit); ++c) {
+          for (int c = part * kSplit; c < (part ? 4 : kSplit); ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const uint32_t* s2 = &sr[c][e * 2];
-              const float s0 = __uint_as_float(s2[0]), s1 = __uint_as_float(s2[1]);
+              const float s0 = __uint_as_float(sr[c][e * 2]), s1 = __uint_as_float(sr[c][e * 2 + 1]);
               float2 w;
               if (decltype(poly)::value && (e * kPoly) / 16 != ((e + 1) * kPoly) / 16) {  // (spread evenly)
                 w = ex2_fma(make_float2(fma_sat(s0, sc128, nm128), fma_sat(s1, sc128, nm128)));
@@ -455,7 +472,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
           tc::tmem_st_wait();
           tc::tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&bars->p_full[I][half]);
+          if (lane == 0) tc::mbar_arrive(&bars->p_full[I][part]);
         }
       };
       if (whole) weights(std::true_type{});
@@ -510,9 +527,19 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, unsigned char* smem
   return true;
 }
 
+// Zeros into the output rows of tiles that do not exist (one warp per CTA, beside the others' work).
+__device__ __forceinline__ void clear_padding(const PromptArgs& a, const int* pre, int lane) {
+  const int rows = a.pair_heads ? kRows : 2 * kRows, per_row = a.Hq * a.D / 8;
+  for (int b = 0; b < a.B; ++b)
+    for (int t = (pre[b + 1] - pre[b]) * rows + (int)blockIdx.x; t < a.T; t += gridDim.x) {
+      uint4* dst = reinterpret_cast<uint4*>(a.out + ((size_t)b * a.T + t) * a.Hq * a.D);
+      for (int i = lane; i < per_row; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+}
+
 }  // namespace
 
-template <int DP>
+template <int DP, bool LISTED>
 __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __grid_constant__ PromptArgs a) {
   extern __shared__ __align__(1024) unsigned char smem[];
   PromptBars* bars = reinterpret_cast<PromptBars*>(smem + PC<DP>::kOffBar);
@@ -540,22 +567,41 @@ __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&bars->tmem_base, 512);
   pdl_wait();
+  int* pre = reinterpret_cast<int*>(smem + PC<DP>::kOffPre);
+  if (LISTED && warp == 0) {  // tiles of every sequence, prefix
+    const int rows = a.pair_heads ? kRows : 2 * kRows;
+    int carry = 0;
+    for (int base = 0; base < a.B; base += 32) {
+      int x = base + lane < a.B ? (max(min(a.lengths[base + lane], a.S) - (a.S - a.T), 0) + rows - 1) / rows : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (base + lane < a.B) pre[base + lane + 1] = x + carry;
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
   tc::tc_fence_before_sync();
   __syncthreads();
   tc::tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
+  const int n_items = LISTED ? __shfl_sync(0xffffffffu, pre[a.B], 0) * (a.units / a.B) : a.n_items;
   bool ok = true;
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    ok = softmax<DP>(a, smem, bars, tmem, warp >> 2, tid & 127, warp & 3, lane);
+    ok = softmax<DP, LISTED>(a, pre, n_items, smem, bars, tmem, warp >> 2, tid & 127, warp & 3, lane);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kProducerWarp) {
-      if (lane == 0) ok = produce<DP>(a, smem, bars);
+      if (lane == 0) ok = produce<DP, LISTED>(a, pre, n_items, smem, bars);
       __syncwarp();
     } else if (warp == kMmaWarp) {
       // (the whole warp walks the tiles: operands that are uniform over it reach the issuing instructions without detours)
-      ok = issue<DP>(a, smem, bars, tmem);
+      ok = issue<DP, LISTED>(a, pre, n_items, smem, bars, tmem);
+    } else if (LISTED && warp == kMmaWarp + 1) {
+      clear_padding(a, pre, lane);
     }
   }
   if (!ok) {
@@ -584,9 +630,9 @@ bool encode_rows(CUtensorMap* m, const Tensor4& t, int batch, int heads, int row
   return encode_bf16_map(m, t.ptr, 4, dims, strides, box);
 }
 
-template <int DP>
+template <int DP, bool LISTED>
 cudaError_t launch_prompt(const PromptArgs& a, int sms, cudaStream_t stream) {
-  auto kern = kvm_window_prompt_kernel<DP>;
+  auto kern = kvm_window_prompt_kernel<DP, LISTED>;
   static std::atomic<unsigned long long> raised{0};
   const cudaError_t e = raise_smem_limit(kern, PC<DP>::kSmem, raised);
   if (e != cudaSuccess) return e;
@@ -619,7 +665,8 @@ cudaError_t window_prompt_dispatch(int D, int batch, int Hq, int Hkv, int T, int
       !encode_rows(&a.mv, v, batch, Hkv, S, D, &a.v_head_inner))
     return cudaErrorInvalidValue;
   const int sms = window_sm_count();
-  return D == 128 ? launch_prompt<128>(a, sms, stream) : launch_prompt<64>(a, sms, stream);
+  if (lengths && batch <= kMaxListed) return D == 128 ? launch_prompt<128, true>(a, sms, stream) : launch_prompt<64, true>(a, sms, stream);
+  return D == 128 ? launch_prompt<128, false>(a, sms, stream) : launch_prompt<64, false>(a, sms, stream);
 }
 
 }  // namespace kvm
