@@ -50,7 +50,7 @@ struct PC {
 };
 
 struct PromptBars {
-  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], pv_done[2], o_final[2], o_free[2];
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], o_final[2], o_free[2];
   uint32_t tmem_base;
 };
 
@@ -240,10 +240,7 @@ struct Issuer {
         for (int s = half * kSplit * 2; s < (half ? 8 : kSplit * 2); ++s)
           tc::mma_ts(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + s * 8, dv + (uint64_t)((pv_slot * PC<DP>::kTileBytes + s * 2048) >> 4),
                      kIdescPv, !first[I] || s > 0);
-        if (half == 1) {
-          tc::mma_commit(&bars->pv_done[I]);
-          if (last[I]) tc::mma_commit(&bars->o_final[I]);
-        }
+        if (half == 1 && last[I]) tc::mma_commit(&bars->o_final[I]);
       }
       __syncwarp();
     }
@@ -304,12 +301,15 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
         if (!is.template qk<0>(ks, done0 == 1, done0 == cnt0)) return false;
       }
       if (!is.template pv<1>()) return false;
-      if (is.slot_held) is.commit(&bars->kv_empty[is.pv_slot]);
       if (it.uses(1, u)) {
         ++done1;
         if (!is.template qk<1>(ks, done1 == 1, done1 == cnt1)) return false;
       }
-      is.commit(&bars->kv_empty[ks]);
+      if (elected()) {
+        if (is.slot_held) tc::mma_commit(&bars->kv_empty[is.pv_slot]);
+        tc::mma_commit(&bars->kv_empty[ks]);
+      }
+      __syncwarp();
       is.pv_slot = vs;
       is.pv_parity = vr;
       is.slot_held = true;
@@ -415,9 +415,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? tmax : m_run;
         const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - m_new);
-        if (done > 0) {  // O may only be touched between P V of the last tile (complete) and of this one (waits for this warp)
-          if (!warp_wait(&bars->pv_done[I], (n - 1) & 1)) return false;
-          tc::tc_fence_after_sync();
+        if (done > 0) {  // (P V of the last tile, issued ahead of these scores, is complete with them; that of this tile waits for this warp)
 #pragma unroll 1
           for (int c = 0; c < DP; c += 16) {
             uint32_t o[16];
@@ -555,7 +553,6 @@ __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __
       tc::mbar_init(&bars->s_full[i], 1);
       tc::mbar_init(&bars->p_full[i][0], 4);
       tc::mbar_init(&bars->p_full[i][1], 4);
-      tc::mbar_init(&bars->pv_done[i], 1);
       tc::mbar_init(&bars->o_final[i], 1);
       tc::mbar_init(&bars->o_free[i], 4);
     }
