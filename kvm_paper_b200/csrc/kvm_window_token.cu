@@ -11,9 +11,9 @@
 // dimension and the query heads on N (8 or 16 columns).
 // 4 bits: the codes become f16 with one conversion instruction per two values.  q is scaled by a power of two per head into
 // f16's range.  A key group's scale multiplies the fp32 sum of its group; a value group's scale multiplies the weights, as
-// f16 relative to a running power of two R above all scales seen so far (the output is rescaled when R rises, as with the
-// softmax maximum): a value scale 2^-24 below the largest of its sequence is lost, which is an error of 2^-24 of that
-// largest value.
+// f16 relative to the largest power of two R in the scales seen so far (the output is rescaled when R rises, as with the
+// softmax maximum).  Weights go up to 2^8 and scales to 2^7, so that the product uses f16 to its top: scales down to 2^-25 R and
+// weights down to 2^-22 of the largest keep all their bits, smaller ones an error of 2^-31 R and 2^-33 of the largest.
 // The new token: the CTA that reads the chunk with its row patches the stage and writes the row to memory.
 #include <algorithm>
 #include <type_traits>
@@ -30,7 +30,8 @@ constexpr int kMaxStages = 8;
 constexpr int kBox = 16;                      // rows per TMA box (16 bits)
 constexpr int kSmemPerSm = 228 * 1024;        // of which every CTA takes 1 KB more than it asks for
 constexpr int kMaxBatch = 1024;               // sequences per launch
-constexpr float kLowest = -3e38f;             // running maximum before the first score
+constexpr float kLowest = -3e38f;             // reference of the weights before the first score
+constexpr unsigned kScaleUp = 6;              // see R below
 
 // How a variant works.  4 bits: bound by the math warps (conversions and fixed latencies), which is why a warp takes T = 4 groups of
 // 16 rows of a chunk side by side; head dimensions below 128 leave the registers for two CTAs per SM.  Short caches of 128
@@ -502,11 +503,13 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
           // the exponent of the largest of them
           const unsigned top = __reduce_max_sync(kAll, max(top2 & 0xffffu, top2 >> 16)) & 0x7f80u;
-          if (top > r_bits + (6u << 7) || (r_bits == 0 && top)) {  // a scale is below 2^7 R, a weight at most 2^8: f16 holds the product
+          if (top > r_bits) {
             r_alpha = r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
             r_bits = top;
           }
-          const float inv = __uint_as_float((254u - (r_bits >> 7)) << 23);
+          // (a scale is below 2 R here, a weight at most 2^8: with 2^6 / R, f16 just holds the product)
+          const unsigned e_r = r_bits >> 7;
+          const float inv = __uint_as_float((254u - e_r + min(e_r, kScaleUp)) << 23);
 #pragma unroll
           for (int u = 0; u < N; ++u)
             if (lane < 8 * NG) vsc[u * 8 * NG + lane] = pack_f16(__uint_as_float(x[u] << 16) * inv, __uint_as_float(x[u] & 0xffff0000u) * inv);
@@ -576,7 +579,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
         }
 
-        // ---- running maximum (raised when a chunk exceeds it by 2^8), weights
+        // ---- weights up to 2^8: the reference m is 8 below the running maximum (f16 holds 2^-24 .. 2^15)
         float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
@@ -596,8 +599,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 16)) * qs[hb][e];  // (positive)
             const bool up = x > m[hb][e] + 8.f;
-            alpha[hb][e] = up ? ex2(m[hb][e] - x) : 1.f;
-            m[hb][e] = up ? x : m[hb][e];
+            alpha[hb][e] = up ? ex2(m[hb][e] - (x - 8.f)) : 1.f;
+            m[hb][e] = up ? x - 8.f : m[hb][e];
           }
         }
         // (always: the FMA pipe is idle, and without a branch the rest of the chunk mixes with it)
@@ -724,7 +727,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         }
         if (head < G) {
           float* dst = ored + ((size_t)warp * G + head) * D;
-          const float up = BITS == 4 ? __uint_as_float(r_bits << 16) : 1.f;
+          const float up = BITS == 4 ? __uint_as_float(r_bits << 16) * __uint_as_float((127u - min(r_bits >> 7, kScaleUp)) << 23) : 1.f;
 #pragma unroll
           for (int k2 = 0; k2 < D / 16; ++k2) {
             // 4 bits: channels 32 (k2/2) + 4 g + 2 (k2%2) + {0, 1};  16 bits: 64 (k2/4) + 8 g + 2 (k2%4) + {0, 1}, and for

@@ -109,8 +109,8 @@ def assert_near(got, want, mag, bits=16, what=""):
     tol = (U_BF16 if bits == 16 else 2 * U_F16) * mag + WEIGHT_NOISE * mag + U_BF16 * want.abs() * (1 + 2.0 ** -6) + 1e-30
     same_nan = torch.isnan(got) == torch.isnan(want)
     assert bool(same_nan.all()), f"{what}: NaN in other places ({int((~same_nan).sum())})"
-    err = torch.where(torch.isnan(want) | (got == want), torch.zeros_like(want), (got - want).abs())
-    worst = (err / tol).nan_to_num(nan=math.inf).max().item() if err.numel() else 0.0
+    fine = torch.isnan(want) | (got == want)
+    worst = torch.where(fine, torch.zeros_like(want), (got - want).abs() / tol).nan_to_num(nan=math.inf).max().item() if got.numel() else 0.0
     assert worst <= 1.0, f"{what}: {worst:.2f} of the tolerance"
 
 
