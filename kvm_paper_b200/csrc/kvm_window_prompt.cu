@@ -15,7 +15,7 @@
 //                          (fp32), P as bf16; behind the last tile O / l to global memory.
 // Infinities and NaN in values that a row does not see: a masked weight is 0, and 0 x inf would reach the row through the
 // product.  Value rows behind a sequence's length are cleared in shared memory; for any other, a row whose sum is finite
-// but whose output is not is computed again by its thread from the keys that it sees (redo_row).
+// but whose output is not is settled by its thread from the keys that it sees (redo_columns).
 // Every wait is bounded; one that runs out sets the status word, and the CTA leaves through its common exit.
 #include <algorithm>
 #include <type_traits>
@@ -319,18 +319,40 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
 }
 
 // ------------------------------------------------------------------------------------------ softmax
-// One query row of which a value that it does not see was an infinity or NaN: the weighted sum over the keys that it sees,
-// with the maximum and the sum that the tiles gave (the weights are not rounded here).
-__device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hkv, int t, int p, float m, float inv) {
-  const bf16* qr = a.q.row(b, hq, t);
-  bf16* dst = a.out + (((size_t)b * a.T + t) * a.Hq + hq) * a.D;
-  const int lo = max(0, p - a.window + 1), ns = min(a.sinks, lo);
-  const float neg_m = m == -INFINITY ? 0.f : -m;
-  for (int c0 = 0; c0 < a.D; c0 += 32) {
-    float acc[32];
+// Columns [c0, c0 + 32) of a query row whose tensor-core sums are not finite in the columns of `bad`, though its scores are: an
+// infinity or NaN among the values, of a key that the row sees or of one that it does not (0 x inf), or sums beyond fp32.  First
+// the values that the row sees are looked through: those columns that hold a NaN or infinity get theirs; what is left is summed
+// again over the keys that the row sees, with the maximum and the sum that the tiles gave and the weights normalised ahead.
+__device__ __noinline__ void redo_columns(const PromptArgs& a, int b, int hq, int hkv, int t, int p, int c0, unsigned bad, float m, float inv) {
+  bf16* dst = a.out + (((size_t)b * a.T + t) * a.Hq + hq) * a.D + c0;
+  const int lo = max(0, p - a.window + 1), ns = min(a.sinks, lo), n = ns + p + 1 - lo;
+  unsigned nan = 0, pos = 0, neg = 0;
+  for (int i = 0; i < n && (bad & ~(nan | (pos & neg))); ++i) {
+    const bf16* vr = a.v.row(b, hkv, i < ns ? i : lo + i - ns) + c0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    for (int i = 0; i < ns + p + 1 - lo; ++i) {
+    for (int e = 0; e < 32; e += 8) {
+      const uint4 y = *reinterpret_cast<const uint4*>(vr + e);
+      const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        const unsigned u = (ys[z >> 1] >> (16 * (z & 1))) & 0xffffu;
+        if ((u & 0x7f80u) != 0x7f80u) continue;
+        const unsigned bit = 1u << (e + z);
+        if (u & 0x7fu) nan |= bit;
+        else if (u & 0x8000u) neg |= bit;
+        else pos |= bit;
+      }
+    }
+  }
+  nan |= pos & neg;
+  const unsigned sum_again = bad & ~(nan | pos | neg);
+  float acc[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+  if (sum_again) {
+    const bf16* qr = a.q.row(b, hq, t);
+    const float neg_m = m == -INFINITY ? 0.f : -m;
+    for (int i = 0; i < n; ++i) {
       const int j = i < ns ? i : lo + i - ns;
       const bf16* kr = a.k.row(b, hkv, j);
       float s = 0.f;
@@ -343,7 +365,7 @@ __device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hk
           s = fmaf(f.x, h.x, fmaf(f.y, h.y, s));
         }
       }
-      const float w = ex2(fmaf(s, a.scale_log2, neg_m));
+      const float w = ex2(fmaf(s, a.scale_log2, neg_m)) * inv;
       const bf16* vr = a.v.row(b, hkv, j) + c0;
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
@@ -357,9 +379,11 @@ __device__ __noinline__ void redo_row(const PromptArgs& a, int b, int hq, int hk
         }
       }
     }
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) *reinterpret_cast<uint32_t*>(dst + c0 + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
   }
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (bad >> i & 1)
+      dst[i] = __float2bfloat16_rn((nan >> i & 1) ? __int_as_float(0x7fffffff) : (pos >> i & 1) ? INFINITY : (neg >> i & 1) ? -INFINITY : acc[i]);
 }
 
 template <int DP, bool LISTED>
@@ -493,16 +517,17 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
     const bool valid = mine && p < it.len;
     if (poison || m_run == -INFINITY) l_run = __int_as_float(0x7fffffff);  // (no score above -inf: 0 / 0)
     const float inv = valid ? 1.0f / l_run : 0.f;
-    bool bad = false;
+    unsigned bad[DP / 32];
 #pragma unroll
     for (int hb = 0; hb < DP / 32; ++hb) {
       uint32_t o[32];
       tc::tmem_ld32(col_o + hb * 32, o);
       tc::tmem_ld_wait();
+      bad[hb] = 0;
       if (hb * 32 < a.D && mine) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          bad |= !(fabsf(__uint_as_float(o[i])) < INFINITY);
+          if (!(fabsf(__uint_as_float(o[i])) < INFINITY)) bad[hb] |= 1u << i;
           o[i] = valid ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
         }
 #pragma unroll
@@ -519,7 +544,11 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
     tc::tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&bars->o_free[I]);
-    if (bad && valid && l_run < INFINITY) redo_row(a, it.b, it.pick(it.hq, I), it.hkv, t, p, m_run, inv);
+    if (valid && l_run < INFINITY) {
+#pragma unroll
+      for (int hb = 0; hb < DP / 32; ++hb)
+        if (bad[hb]) redo_columns(a, it.b, it.pick(it.hq, I), it.hkv, t, p, hb * 32, bad[hb], m_run, inv);
+    }
     __syncwarp();
   }
   return true;

@@ -579,7 +579,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
         }
 
-        // ---- weights up to 2^8: the reference m is 8 below the running maximum (f16 holds 2^-24 .. 2^15)
+        // ---- weights up to 2^kTop: the reference m is that much below the running maximum (4 bits: f16 holds 2^-24 .. 2^15)
+        constexpr float kTop = BITS == 4 ? 8.f : 0.f;
         float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
@@ -598,9 +599,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 16)) * qs[hb][e];  // (positive)
-            const bool up = x > m[hb][e] + 8.f;
-            alpha[hb][e] = up ? ex2(m[hb][e] - (x - 8.f)) : 1.f;
-            m[hb][e] = up ? x - 8.f : m[hb][e];
+            const bool up = x > m[hb][e] + kTop;
+            alpha[hb][e] = up ? ex2(m[hb][e] - (x - kTop)) : 1.f;
+            m[hb][e] = up ? x - kTop : m[hb][e];
           }
         }
         // (always: the FMA pipe is idle, and without a branch the rest of the chunk mixes with it)

@@ -451,3 +451,34 @@ def test_many_sequences_and_repeated_calls():
             ref.write(b, k[b, :, :lens[b]], v[b, :, :lens[b]], 0)
             want, mag = ref.attend(b, q[b], lens[b])
             wh.assert_near(got[b, 0], want.flatten(), mag.flatten(), bits, f"{b}")
+
+
+def test_prompt_values_near_the_largest_number():
+    """Sums of weights that are not normalised yet would pass the range of fp32; the output does not."""
+    from kvm_paper_b200 import window
+    g = _gen(31)
+    T = 300
+    q, k = wh.heads_data(g, 1, 2, T, 64), wh.heads_data(g, 1, 1, T, 64)
+    v = wh.heads_data(g, 1, 1, T, 64)
+    v[..., :40] = 3e38
+    v[..., 40:44] *= 1e37
+    got = window.window_attention(q, k, v, window=100, sinks=1).view(1, T, 2, 64)
+    want, mag = wh.prompt(q, k, v, 100, 1)
+    assert bool(torch.isfinite(got).all())
+    wh.assert_near(got, want, mag)
+
+
+def test_prompt_of_nothing_but_nan_ends_soon():
+    """Every value NaN: every row is looked at again, and settled by the first key that it sees."""
+    from kvm_paper_b200 import window
+    g = _gen(32)
+    T = 8192
+    q, k = wh.heads_data(g, 1, 4, T, 128), wh.heads_data(g, 1, 2, T, 128)
+    v = torch.full((1, 2, T, 128), math.nan, device="cuda", dtype=torch.bfloat16)
+    window.window_attention(q, k, v, window=None)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got = window.window_attention(q, k, v, window=None)
+    end.record()
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(got).all()) and start.elapsed_time(end) < 50.0
