@@ -214,11 +214,31 @@ __device__ __forceinline__ bool produce(const PromptArgs& a, const int* pre, int
 // the next) while the other is in its softmax.  (Two issuing threads interleave on the tensor core: both tiles' scores then
 // come late and together, both softmaxes run at the same time, and the tensor core idles meanwhile.)  Step u: P V of
 // tile u - 1 and Q K of tile u, for query tile 0, then for 1; it goes on from item to item.
+// The issuing warp is the narrowest part of the pipeline: operand descriptors differ in the low word's address field only (no
+// carry leaves it), so that an MMA costs one 32-bit addition per operand.
+__device__ __forceinline__ void mma_ss_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+      :
+      : "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+      :
+      : "r"(d), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
 template <int DP>
 struct Issuer {
   static constexpr uint32_t kIdescQk = tc::make_idesc(kRows, kRows, 0, 0), kIdescPv = tc::make_idesc(kRows, DP, 0, 1);
+  static constexpr uint32_t kTile = PC<DP>::kTileBytes >> 4;
   PromptBars* bars;
-  uint64_t dq, dk, dv;
+  uint32_t dq, dk, dv, hi;  // low words of the first query tile's, slot 0's key and value descriptors; the high word
   uint32_t tmem;
   int n[2] = {0, 0}, nq[2] = {0, 0};   // tiles whose P V is issued, items begun
   bool pending[2] = {false, false}, first[2], last[2];
@@ -231,6 +251,7 @@ struct Issuer {
     pending[I] = false;
     if (first[I] && nq[I] > 1 && !warp_wait(&bars->o_free[I], (nq[I] - 2) & 1)) return false;  // the last item's output has been read
     if (!warp_wait(&bars->kv_full[pv_slot], pv_parity)) return false;
+    const uint32_t v_lo = dv + pv_slot * kTile;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (!warp_wait(&bars->p_full[I][half], n[I] & 1)) return false;
@@ -238,8 +259,7 @@ struct Issuer {
       if (elected()) {
 #pragma unroll
         for (int s = half * kSplit * 2; s < (half ? 8 : kSplit * 2); ++s)
-          tc::mma_ts(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + s * 8, dv + (uint64_t)((pv_slot * PC<DP>::kTileBytes + s * 2048) >> 4),
-                     kIdescPv, !first[I] || s > 0);
+          mma_ts_lo(tmem + PC<DP>::kColO + I * DP, tmem + I * 128 + s * 8, v_lo + s * (2048 >> 4), hi, kIdescPv, !first[I] || s > 0);
         if (half == 1 && last[I]) tc::mma_commit(&bars->o_final[I]);
       }
       __syncwarp();
@@ -253,13 +273,13 @@ struct Issuer {
       if (!warp_wait(&bars->q_full[I], nq[I] & 1)) return false;
       ++nq[I];
     }
+    const uint32_t k_lo = dk + k_slot * kTile;
     tc::tc_fence_after_sync();
     if (elected()) {
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
-        const uint64_t off = (uint64_t)(((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4);
-        tc::mma_ss(tmem + I * 128, dq + (uint64_t)((I * PC<DP>::kTileBytes) >> 4) + off, dk + (uint64_t)((k_slot * PC<DP>::kTileBytes) >> 4) + off,
-                   kIdescQk, s > 0);
+        const uint32_t off = ((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4;
+        mma_ss_lo(tmem + I * 128, dq + I * kTile + off, k_lo + off, hi, kIdescQk, s > 0);
       }
       tc::mma_commit(&bars->s_full[I]);
       if (is_last) tc::mma_commit(&bars->q_empty[I]);
@@ -281,9 +301,11 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
   Issuer<DP> is;
   is.bars = bars;
   is.tmem = tmem;
-  is.dq = tc::make_desc(tc::smem_u32(smem), 16, 1024);
-  is.dk = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
-  is.dv = tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);
+  const uint64_t d0 = tc::make_desc(tc::smem_u32(smem), 16, 1024);
+  is.dq = (uint32_t)d0;
+  is.hi = (uint32_t)(d0 >> 32);
+  is.dk = (uint32_t)tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), 16, 1024);
+  is.dv = (uint32_t)tc::make_desc(tc::smem_u32(smem + PC<DP>::kOffKv), kRows * 128, 1024);  // (the high words are alike)
   int slot = 0, round = 0;
   for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
     const Item<LISTED> it(a, pre, x);
