@@ -263,7 +263,7 @@ int check_window(const kvm_window_cache* c, bool arrays) {
 }
 
 int check_scale(float scale) {
-  if (!(scale > 0.f && scale < 3e38f)) return fail(KVM_ERR_BAD_ARGUMENT, "scale %g must be positive and finite", (double)scale);
+  if (!(scale > 0.f && scale < 1e38f)) return fail(KVM_ERR_BAD_ARGUMENT, "scale %g must be positive and below 1e38", (double)scale);
   return KVM_OK;
 }
 

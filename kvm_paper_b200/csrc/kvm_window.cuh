@@ -36,15 +36,6 @@ struct WindowDev {
   __host__ __device__ __forceinline__ int row_of(int t) const { return t < sinks ? t : sp + (t - sinks) % ring; }
   // rows [0, live) are looked at for a sequence of n tokens
   __host__ __device__ __forceinline__ int live(int n) const { return n <= 0 ? 0 : (n <= sinks ? n : sp + min(ring, n - sinks)); }
-  // does row r hold a token that the last of n tokens sees?
-  __device__ __forceinline__ bool visible(int r, int n) const {
-    if (r < sp) return r < min(sinks, n);
-    const int m = n - sinks;  // tokens that went through the ring
-    if (m <= 0) return false;
-    int age = (m - 1) % ring - (r - sp);
-    if (age < 0) age += ring;
-    return age < min(window, m);
-  }
 };
 
 // Lengths (or positions) of a batch: a device array, or one number for all.

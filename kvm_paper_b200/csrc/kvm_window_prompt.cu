@@ -126,10 +126,12 @@ struct Item {
   __device__ __forceinline__ int count(int i) const { return pick(end, i) > 0 ? n_sink + pick(end, i) - pick(begin, i) : 0; }
 };
 
-// Bounded wait without pauses between the tries: the roles hand tiles to each other several times per microsecond, and a
-// pause that overshoots is on the path of both.
+// Bounded wait without pauses of its own between the tries: the roles hand tiles to each other several times per microsecond,
+// and a pause that overshoots is on the path of both.  What is waited for comes within microseconds, but for a softmax warp that
+// looks through its rows' values again (redo_columns: up to 1.1 s behind 65536 keys).  A try that fails has waited for about
+// 2700 clocks: 2^26 of them are some 100 s.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 22); ++i)
+  for (uint32_t i = 0; i < (1u << 26); ++i)
     if (tc::mbar_try_wait(bar, parity)) return true;
   return false;
 }
@@ -620,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvm_window_prompt_kernel(const __
     const int rows = a.pair_heads ? kRows : 2 * kRows;
     int carry = 0;
     for (int base = 0; base < a.B; base += 32) {
-      int x = base + lane < a.B ? (max(min(a.lengths[base + lane], a.S) - (a.S - a.T), 0) + rows - 1) / rows : 0;
+      int x = base + lane < a.B ? (max(min(max(a.lengths[base + lane], 0), a.S) - (a.S - a.T), 0) + rows - 1) / rows : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, d);

@@ -60,7 +60,7 @@ kvm_window_write_kernel(WindowDev W, Tensor4 k, Tensor4 v, int n_tokens, SeqInts
   const int b = kvrow / W.Hkv, h = kvrow % W.Hkv;
   const int pos = positions.at(b), len = min(lengths.at(b), n_tokens);
   const int base = (int)blockIdx.x * Piece<D>::kTile;
-  if (pos < 0 || base >= len) return;
+  if (pos < 0 || base >= len || pos > 0x7fffffff - len) return;  // (positions that are not representable: left alone)
   const int first = pos + len - W.ring;  // tokens from there on stay in the ring (positions stay below 2^31)
   if (pos + base >= W.sinks && (long long)pos + base + Piece<D>::kTile <= first) return;
   const Piece<D> at;

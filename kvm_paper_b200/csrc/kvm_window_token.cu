@@ -104,7 +104,7 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMathWarps * 32) : "memory"); }
 
-// Which rows the last of n tokens sees (WindowDev::visible without its division).
+// Which rows the last of n tokens sees: of the ring those whose token is less than `limit` behind the newest.
 struct Seen {
   int sinks, sp, live, newest, ring, limit;
   __device__ __forceinline__ Seen(const WindowDev& W, int n) {
@@ -142,11 +142,10 @@ __host__ __device__ inline size_t partial_floats(int D, int G) { return (size_t)
 
 // The split of the list, the same in both kernels.  whole_rows: ranges end between kv rows.
 struct Split {
-  int total, per, active;  // units (chunks, or kv rows) of the list, per CTA, CTAs with work
+  int total, per;  // units (chunks, or kv rows) of the list, per CTA
   __device__ __forceinline__ Split(int units, int grid) {
     total = units;
     per = max(1, (units + grid - 1) / grid);
-    active = (units + per - 1) / per;
   }
 };
 
@@ -783,7 +782,8 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
   __shared__ float red[2][8];
   __shared__ float2 part[256];
   const int tid = threadIdx.x, head = blockIdx.y;
-  // (the main kernel lets this one start once its own wait is over: the lengths may be read ahead of its end)
+  // The main kernel lets this one start once its own wait is over: the lengths may be read ahead of its end.  Blocks without
+  // work wait for it all the same: what follows in the stream waits for this grid, and through it for the main one.
   build_prefix(W, lens, extra, chunk, b0, nb, pre, tid, 256);
   float* weight = reinterpret_cast<float*>(pre + 2 * nb + 1);
   const int Hkv = W.Hkv;
@@ -796,18 +796,18 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
     row0 = pre[b] * Hkv + h * nc;
   } else {
     const int f = ((int)blockIdx.x + 1) * sp.per;
-    if (f >= sp.total) return;
+    if (f >= sp.total) return pdl_wait();
     b = find_seq(pre, nb, Hkv, f);
     nc = pre[b + 1] - pre[b];
     const int rem = f - pre[b] * Hkv;
     h = rem / nc;
     row0 = f - rem % nc;
-    if (row0 / sp.per != (int)blockIdx.x) return;  // another boundary's
+    if (row0 / sp.per != (int)blockIdx.x) return pdl_wait();  // another boundary's
   }
-  if (nc == 0) return;
+  if (nc == 0) return pdl_wait();
   const int c0 = row0 / sp.per, c1 = (row0 + nc - 1) / sp.per, n = c1 - c0 + 1;  // CTAs that hold parts of the row
-  if (n < 2) return;
   pdl_wait();
+  if (n < 2) return;
   // the row begins in CTA c0 (its second partial result) and goes on in the others (their first)
   auto src = [&](int i) { return partial + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * partial_floats(D, G) + (size_t)head * (D + 2); };
   float mx = kLowest;

@@ -75,6 +75,13 @@ def _counts(x, name: str, batch: int, dev, least: int, most: int):
     return None, x
 
 
+def _int32(x, name: str) -> int:
+    x = int(x)
+    if not -2**31 <= x < 2**31:  # (ctypes would cut it off)
+        raise ValueError(f"{name} must be a 32-bit integer, got {x}")
+    return x
+
+
 def _output(out, like: torch.Tensor, shape) -> torch.Tensor:
     if out is None:
         return like.new_empty(shape)
@@ -85,8 +92,8 @@ def _output(out, like: torch.Tensor, shape) -> torch.Tensor:
 
 def _scale(scale, head_dim: int) -> float:
     s = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not 0.0 < s < 3e38:
-        raise ValueError(f"scale must be positive and finite, got {s}")
+    if not 0.0 < s < 1e38:  # (log2(e) times it is finite in fp32, too)
+        raise ValueError(f"scale must be positive and below 1e38, got {s}")
     return s
 
 
@@ -122,8 +129,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
             raise ValueError(f"lengths must be an int32 tensor, got {type(lengths)}")
         lens, _ = _counts(lengths, "lengths", B, dev, 0, S)
     y = _output(out, q, (B, T, Hq * D))
-    args = _lib.KvmWindowPromptArgs(*qa[:4], *ka[:4], *va[:4], lens, y.data_ptr(), T, S, max(S, 1) if window is None else int(window),
-                                    int(sinks), B, Hq, Hkv, D, _scale(scale, D))
+    args = _lib.KvmWindowPromptArgs(*qa[:4], *ka[:4], *va[:4], lens, y.data_ptr(), T, S, max(S, 1) if window is None else _int32(window, "window"),
+                                    _int32(sinks, "sinks"), B, Hq, Hkv, D, _scale(scale, D))
     _call(dev, _lib.load().kvm_window_attention, C.addressof(args))
     return y
 
@@ -136,8 +143,8 @@ class WindowCache:
     one cache run in the order of their streams; a call that writes must not overlap with another call on the same cache."""
 
     def __init__(self, batch: int, n_kv_heads: int, head_dim: int, *, window: int, sinks: int = 0, bits: int = 16, device="cuda"):
-        self.batch, self.n_kv_heads, self.head_dim = int(batch), int(n_kv_heads), int(head_dim)
-        self.window, self.sinks, self.bits = int(window), int(sinks), int(bits)
+        self.batch, self.n_kv_heads, self.head_dim = _int32(batch, "batch"), _int32(n_kv_heads, "n_kv_heads"), _int32(head_dim, "head_dim")
+        self.window, self.sinks, self.bits = _int32(window, "window"), _int32(sinks, "sinks"), _int32(bits, "bits")
         dev = torch.device(device)
         if dev.type != "cuda":
             raise RuntimeError("kvm_b200 runs on CUDA devices only (there is no CPU path)")

@@ -482,3 +482,84 @@ def test_prompt_of_nothing_but_nan_ends_soon():
     end.record()
     torch.cuda.synchronize()
     assert bool(torch.isnan(got).all()) and start.elapsed_time(end) < 50.0
+
+
+def test_lengths_and_positions_outside_their_range_touch_nothing():
+    """Device numbers that no call may bring: negative lengths count as 0, positions that cannot be held leave their sequence alone."""
+    from kvm_paper_b200 import window
+    g = _gen(33)
+    lowest, highest = -2**31, 2**31 - 1
+    q, k, v = wh.heads_data(g, 4, 2, 40, 64), wh.heads_data(g, 4, 1, 300, 64), wh.heads_data(g, 4, 1, 300, 64)
+    got = window.window_attention(q, k, v, window=50, lengths=_ints([lowest, -1, 300, highest]))
+    want, mag = wh.prompt(q, k, v, 50, 0, lengths=[0, 0, 300, 300])
+    wh.assert_near(got.view(4, 40, 2, 64), want, mag)
+    for bits in (4, 16):
+        c = window.WindowCache(4, 1, 64, window=32, sinks=3, bits=bits)
+        c.write(k[:, :, :5], v[:, :, :5], 0)
+        before = c.read(5)
+        c.write(k[:, :, 5:9], v[:, :, 5:9], _ints([lowest, -1, highest, highest - 3]))
+        c.write(k[:, :, 5:9], v[:, :, 5:9], 5, lengths=_ints([lowest, -1, 0, -5]))
+        y = c.step(q[:, :, :1], k[:, :, 9:10], v[:, :, 9:10], _ints([lowest, -1, -2, highest]))
+        assert not y.any()
+        assert all(torch.equal(a, b) for a, b in zip(c.read(5), before))
+        assert not any(t.any() for t in c.read(_ints([lowest, -1, 0, -7])))
+        assert not c.attend(q[:, :, :1], _ints([lowest, -1, 0, -7])).any()
+    window.check_status()
+
+
+def test_prompts_of_more_sequences_than_are_listed():
+    from kvm_paper_b200 import window
+    g = _gen(34)
+    B, T = 601, 150
+    lens = [(61 * i) % (T + 1) for i in range(B)]
+    q, k, v = wh.heads_data(g, B, 2, T, 32), wh.heads_data(g, B, 1, T, 32), wh.heads_data(g, B, 1, T, 32)
+    want, mag = wh.prompt(q, k, v, 40, 2, lengths=lens)
+    for b, n in enumerate(lens):
+        k[b, :, n:], v[b, :, n:] = math.nan, math.inf
+    got = window.window_attention(q, k, v, window=40, sinks=2, lengths=_ints(lens))
+    wh.assert_near(got.view(B, T, 2, 32), want, mag)
+
+
+def test_short_rows_of_a_long_cache_are_complete_for_what_follows():
+    """No row is cut although the cache's length asks for the joining launch: what follows in the stream sees the output."""
+    from kvm_paper_b200 import window
+    g = _gen(35)
+    c = window.WindowCache(1, 4, 128, window=200000, bits=4)
+    k, v = wh.heads_data(g, 1, 4, 300, 128), wh.heads_data(g, 1, 4, 300, 128)
+    c.write(k, v, 0)
+    q = wh.heads_data(g, 1, 16, 1, 128)
+    want = c.attend(q, 300).clone()
+    out = torch.empty_like(want)
+    for _ in range(200):
+        out.fill_(math.nan)
+        c.attend(q, 300, out=out)
+        assert torch.equal(out.clone(), want)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_first_calls_of_a_process_may_be_captured(bits):
+    import subprocess
+    import sys
+    code = f"""
+import torch
+from kvm_paper_b200 import window
+q = torch.randn(2, 4, 20, 64, device="cuda").bfloat16()
+k = torch.randn(2, 2, 20, 64, device="cuda").bfloat16()
+c = window.WindowCache(2, 2, 64, window=100000, sinks=4, bits={bits})
+pos = torch.full((2,), 20, device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = window.window_attention(q, k, k, window=8, sinks=1)
+    c.write(k, k, 0)
+    z = c.step(q[:, :, :1], k[:, :, :1], k[:, :, :1], pos)
+    a, b = c.read(21)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, window.window_attention(q, k, k, window=8, sinks=1))
+assert torch.equal(z, c.step(q[:, :, :1], k[:, :, :1], k[:, :, :1], pos))
+assert all(torch.equal(s, t) for s, t in zip((a, b), c.read(21)))
+window.check_status()
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -99,3 +99,15 @@ def test_python_calls_refuse_the_cpu():
         window.window_attention(q[0], q, q, window=4)
     with pytest.raises(ValueError, match="tensor"):
         window.window_attention(None, q, q, window=4)
+
+
+@pytest.mark.parametrize("kw", [dict(batch=2**32 + 1), dict(window=2**32 + 8), dict(sinks=-2**32 + 1), dict(head_dim=2**32 + 64), dict(bits=2**32 + 4)])
+def test_numbers_beyond_32_bits_are_refused(kw):
+    with pytest.raises(ValueError, match="32-bit"):
+        window.WindowCache(**{**dict(batch=1, n_kv_heads=2, head_dim=64, window=8), **kw})
+
+
+def test_scales_beyond_the_range_are_refused():
+    lib, c = _lib.load(), _cache()
+    a = _lib.KvmWindowAttendArgs(C.addressof(c), 256, 128, 64, 64, None, 0, 0, 0, None, 0, 0, 0, None, 256, None, 0, 2, 4, 2.9e38)
+    assert lib.kvm_window_attend(C.addressof(a), None) == 1 and "scale" in _err()
