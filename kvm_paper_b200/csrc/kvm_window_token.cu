@@ -556,7 +556,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
               }
             }
           } else {
-            const int r = warp * 16 + g;
+            const int r = (warp + (u0 + u) * kMathWarps) * 16 + g;
 #pragma unroll
             for (int blk = 0; blk < GM::kBlocks; ++blk) {
               constexpr int PIECES = GM::kBoxW / 32;  // 16-byte pieces per thread and row: 2 (64 channels) or 1
@@ -679,7 +679,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
               uint32_t x[4][WORDS];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const int rr = warp * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
+                const int rr = (warp + (u0 + u) * kMathWarps) * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
                 lds(x[r], D >= 64 ? vb + blk * (CH * 128) + rr * 128 + ((g ^ (rr & 7)) << 4) : vb + rr * 64 + g * 8);
                 if (seen_rows != kWhole && !((vis(u0 + u) >> (rr & 15)) & 1)) {  // (0 x NaN)
 #pragma unroll
@@ -929,7 +929,7 @@ template <typename F>
 auto token_variant(int D, int bits, const WindowDev& W, int G, F f) {
   auto heads = [&](auto d, auto h) {
     constexpr int kD = decltype(d)::value, kH = decltype(h)::value;
-    if (bits == 16) return f(TokLaunch<TokGeom<kD, 16, kH, 1>>{});
+    if (bits == 16) return f(TokLaunch<TokGeom<kD, 16, kH, 128 / kD>>{});
     if constexpr (kD == 128 && kH == 1) {
       if (W.rows <= kShortRows) return f(TokLaunch<TokGeom<kD, 4, kH, 2>>{});
     }
