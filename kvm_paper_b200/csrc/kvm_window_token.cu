@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kMathWarps = 8;
 constexpr int kMaxStages = 8;
-constexpr int kBox = 16;                      // rows per TMA box (16 bits)
+constexpr int kBox = 128;                     // rows per TMA box (16 bits; the end of a cache comes in boxes of 16)
 constexpr int kSmemPerSm = 228 * 1024;        // of which every CTA takes 1 KB more than it asks for
 constexpr int kMaxBatch = 1024;               // sequences per launch
 constexpr float kLowest = -3e38f;             // reference of the weights before the first score
@@ -71,7 +71,7 @@ struct TokSmem {
 };
 
 struct TokMaps {
-  CUtensorMap k, v;  // [all rows][D], boxes of 16 rows
+  CUtensorMap k, v, k_end, v_end;  // [all rows][D], boxes of kBox rows, of 16 rows
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -325,10 +325,12 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         tc::bulk_g2s(st, W.blocks + (kvrow * (W.rows / 16) + (size_t)pp.c * (CH / 16)) * Block4<D>::kBytes, groups * Block4<D>::kBytes, &full[s]);
     } else {
       const int y = (int)(kvrow * W.rows) + pp.c * CH;  // (all rows of a cache: below 2^31, checked on the host)
-      for (int j = lane; j < groups * GM::kBlocks * 2; j += 32) {
-        const int half = j / (groups * GM::kBlocks), k2 = j % (groups * GM::kBlocks), blk = k2 / groups, gr = k2 % groups;
-        tc::tma_load_2d(st + half * (CH * D * 2) + blk * (CH * GM::kBoxW * 2) + gr * (kBox * GM::kBoxW * 2), half ? &maps.v : &maps.k,
-                        blk * GM::kBoxW, y + gr * kBox, &full[s]);
+      const int large = groups / (kBox / 16), boxes = large + groups % (kBox / 16);
+      for (int j = lane; j < boxes * GM::kBlocks * 2; j += 32) {
+        const int half = j / (boxes * GM::kBlocks), k2 = j % (boxes * GM::kBlocks), blk = k2 / boxes, box = k2 % boxes;
+        const int row = min(box, large) * kBox + max(box - large, 0) * 16;
+        tc::tma_load_2d(st + half * (CH * D * 2) + (blk * CH + row) * (GM::kBoxW * 2),
+                        box < large ? (half ? &maps.v : &maps.k) : (half ? &maps.v_end : &maps.k_end), blk * GM::kBoxW, y + row, &full[s]);
       }
     }
     if (first && lane < G) tc::bulk_g2s(st + lay.q + lane * D * 2, q.row(b0 + pp.b, pp.h * G + lane, 0), D * 2, &full[s]);
@@ -889,8 +891,9 @@ struct TokLaunch {
     if (BITS == 16) {
       const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)W.batch * W.Hkv * W.rows};
       const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-      const cuuint32_t box[2] = {(cuuint32_t)GM::kBoxW, (cuuint32_t)kBox};
-      if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box))
+      const cuuint32_t box[2] = {(cuuint32_t)GM::kBoxW, (cuuint32_t)kBox}, end[2] = {(cuuint32_t)GM::kBoxW, 16};
+      if (!encode_bf16_map(&maps.k, W.k, 2, dims, strides, box) || !encode_bf16_map(&maps.v, W.v, 2, dims, strides, box) ||
+          !encode_bf16_map(&maps.k_end, W.k, 2, dims, strides, end) || !encode_bf16_map(&maps.v_end, W.v, 2, dims, strides, end))
         return cudaErrorInvalidValue;
     }
     auto kern = kvm_window_token_kernel<GM>;
