@@ -38,7 +38,9 @@ constexpr unsigned kScaleUp = 6;              // see R below
 // channels are bound by the changes from kv row to kv row, which two CTAs with smaller chunks (T = 2) overlap: 64 x 8 kv
 // rows of 516 tokens 19.9 us against 26.6, 8 x 16 of 4096 25.9 against 23.2 (see kShortRows).  The copies, one per chunk, are
 // issued by math warp 0.
-// 16 bits: bound by memory: one CTA with deep stages and a producer warp of its own (many copies per chunk).
+// 16 bits: bound by memory (64 x 4 kv rows of 4100 x 128, 4 query heads each: 84 us, 6.4 TB/s): one CTA, chunks of 64 KB at every
+// head dimension, copied in boxes of 128 rows (of 16 rows throughout: 97 us; 64 x 8 of 4100 x 32: 48 us against 83) by a
+// producer warp of its own (by math warp 0: 64 x 16 of 516 x 128 54 us against 46).
 template <int D_, int BITS_, int NH_, int T_>
 struct TokGeom {
   static constexpr int D = D_, BITS = BITS_, NH = NH_;           // NH: blocks of 8 query heads per kv head
