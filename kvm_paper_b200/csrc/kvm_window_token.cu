@@ -38,7 +38,7 @@ constexpr unsigned kScaleUp = 6;              // see R below
 // channels are bound by the changes from kv row to kv row, which two CTAs with smaller chunks (T = 2) overlap: 64 x 8 kv
 // rows of 516 tokens 19.9 us against 26.6, 8 x 16 of 4096 25.9 against 23.2 (see kShortRows).  The copies, one per chunk, are
 // issued by math warp 0.
-// 16 bits: bound by memory (64 x 4 kv rows of 4100 x 128, 4 query heads each: 84 us, 6.4 TB/s): one CTA, chunks of 64 KB at every
+// 16 bits: bound by memory (64 x 4 kv rows of 4100 x 128, 4 query heads each: 80 us, 6.7 TB/s): one CTA, chunks of 64 KB at every
 // head dimension, copied in boxes of 128 rows (of 16 rows throughout: 97 us; 64 x 8 of 4100 x 32: 48 us against 83) by a
 // producer warp of its own (by math warp 0: 64 x 16 of 516 x 128 54 us against 46).
 template <int D_, int BITS_, int NH_, int T_>
@@ -864,14 +864,21 @@ struct TokPlan {
     while (n > 16 && TokSmem(GM{}, G, n, 2).total > limit) n -= 16;
     return n;
   }
-  // Whole kv rows per CTA where cutting them gains less than the second launch and the partial results cost (about 2.5 us;
-  // a chunk streams in about its bytes / 44 GB/s per SM).
+  // Whole kv rows per CTA where cutting them gains less than it costs.  Fitted to both ways of 170 calls (1 to 64 sequences of
+  // 256 to 16384 tokens, all variants): a chunk takes about 1.7 us (4 bits) or 0.8 us (16 bits), all of them together no less
+  // than their bytes at 6.5 TB/s; cutting costs 2.5 us for the second launch (taken as 3.5: outside a graph the host needs 4 us
+  // for it) and 2.5 more where a CTA's share covers more than a chunk and so, as a rule, parts of two rows.  8 sequences of 512
+  // tokens with 16 heads x 128, 4 bits: 9.1 us whole, 12.4 cut; of 16384 with 4 heads: 73 whole, 26 cut.  The rule's choices
+  // take 1 % more than the better ones in sum, 20 % at worst (16 bits, 8 x 2048 tokens, 8 heads x 128: 16.2 for 13.4).
   template <typename GM>
   static bool whole_rows(const WindowDev& W, int nb, int ctas) {
     const int max_chunks = (W.rows + GM::kChunk - 1) / GM::kChunk;
-    const long long rows = (long long)nb * W.Hkv, chunks = rows * max_chunks;
-    const double chunk_us = GM::kStageKv / 44e3 * GM::kCtas;
-    return (double)((rows + ctas - 1) / ctas) * max_chunks * chunk_us <= (double)((chunks + ctas - 1) / ctas) * chunk_us + 2.5;
+    const long long rows = (long long)nb * W.Hkv, chunks = rows * max_chunks, per = (chunks + ctas - 1) / ctas;
+    const double chunk_us = GM::BITS == 4 ? 1.7 : 0.8, copy_us = GM::kStageKv / 6.5e6;
+    // (rounds of a row per CTA: the last one may leave CTAs, and the memory, idle)
+    const long long rounds = rows / ctas, rest = rows % ctas;
+    const double whole = max_chunks * (rounds * std::max(chunk_us, ctas * copy_us) + (rest ? std::max(chunk_us, rest * copy_us) : 0.0));
+    return whole <= std::max(per * chunk_us, chunks * copy_us) + (per > 1 ? 5.0 : 3.5);
   }
 };
 
