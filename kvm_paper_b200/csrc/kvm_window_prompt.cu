@@ -8,7 +8,7 @@
 //
 //   producer (1 warp)      one thread: tiled TMA copies of the query tiles and, through a ring of slots, of K0, V0, K1, ...
 //   MMA (1 warp)           one thread: S = Q K^T into tensor memory; O += P V with P as the tensor-memory A operand, in two
-//                          parts (96 and 32 keys) as the softmax delivers them.  P lies over the scores it came from, so the next
+//                          parts (64 keys each) as the softmax delivers them.  P lies over the scores it came from, so the next
 //                          scores follow behind P V; while one tile is in its softmax the other has the tensor core.
 //   softmax (4 warps per tile)  one query row per thread: scores from tensor memory, mask (only where a tile is not seen
 //                          whole), running maximum (raised, and O rescaled, when a tile exceeds it by 2^8), exp2, row sum
@@ -17,6 +17,13 @@
 // product.  Value rows behind a sequence's length are cleared in shared memory; for any other, a row whose sum is finite
 // but whose output is not is settled by its thread from the keys that it sees (redo_columns).
 // Every wait is bounded; one that runs out sets the status word, and the CTA leaves through its common exit.
+//
+// Measured (32 / 8 heads x 128, 8192 queries over all earlier tokens): 461 us, 1190 TFLOP/s; 2 x 32768 queries, 16 heads x 128,
+// window 4096: 1.86 ms (2.15 ms in a long run, at the power limit of 1000 W and 1.5 GHz); 64 channels, 2 x 8192 queries, 16 / 4
+// heads, window 2048: 185 us, 650 TFLOP/s.  With a constant in place of the softmax the first takes 443 us: what bounds it is the tensor
+// core (1024 of about 1400 clocks per 128 x 128 tile; its operands and the copies share the bandwidth of shared memory) and the
+// hand-overs to the issuing warp, at 64 channels the hand-overs and the exponentials (52 % of the special-function unit).  One issuing warp
+// with uniform operands instead of one thread: 615 -> 472 us; registers 208 / 88 instead of 224 / 56, which spills: 712 -> 615.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,8 +39,8 @@ constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr float kRescale = 8.0f;  // log2 units
 constexpr int kMaxListed = 500;   // sequences of a batch of unequal lengths whose tiles are listed
-constexpr int kSplit = 3;         // of 4 x 32 keys, those whose weights are handed to the MMA warp first
-constexpr int kPoly = 4;          // of 16 pairs of weights, those formed by polynomial
+constexpr int kSplit = 2;         // of 4 x 32 keys, those whose weights are handed to the MMA warp first (2: 461 us, 3: 465)
+constexpr int kPoly = 4;          // of 16 pairs of weights, those formed by polynomial (none: 487 us, 4: 475, 8: 493)
 constexpr int kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split above the block's registers");
 
@@ -66,7 +73,8 @@ struct PromptArgs {
 };
 
 // What an item is, computed alike by every role.  LISTED: batches of unequal lengths, whose items are the tiles that exist, found
-// through a prefix over the sequences (a template: the few registers cost the others 2 %).
+// through a prefix over the sequences (6 padded prompts of up to 2011 tokens, 64 channels: 46 us against 72; a template: the
+// few registers cost the others 2 %).  The prefix of larger batches would take too much shared memory from the tiles.
 template <bool LISTED>
 struct Item {
   int b, hkv, len, lo, s_end, n_sink, n_tiles;  // first window key, end of the sinks before it, their tiles, tiles in all
