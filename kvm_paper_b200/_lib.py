@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkvm_b200.so")
@@ -116,6 +117,14 @@ class KvmWindowPromptArgs(C.Structure):
     _fields_ = [*_tensor_fields("q"), *_tensor_fields("k"), *_tensor_fields("v"), ("lengths_dev", C.c_void_p), ("out", C.c_void_p),
                 ("n_queries", C.c_int64), ("n_keys", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64), ("batch", C.c_int32),
                 ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
+
+
+def packer(cls):
+    """``pack(*fields) -> bytes`` for an argument block: what ``cls(*fields)`` holds (addresses as integers, 0 for NULL), in a fifth of
+    the time; passed where a call takes the block's address."""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_size_t: "N", C.c_int32: "i", C.c_float: "f"}
+    form = "@" + "".join(code[t] for _, t in cls._fields_)
+    return struct.Struct(form + "x" * (C.sizeof(cls) - struct.calcsize(form))).pack
 
 
 EXPORTS = [

@@ -25,6 +25,7 @@ import torch
 from . import _lib
 from .ops import _stream_ptr
 
+_pack_write, _pack_attend, _pack_prompt = (_lib.packer(c) for c in (_lib.KvmWindowWriteArgs, _lib.KvmWindowAttendArgs, _lib.KvmWindowPromptArgs))
 MAX_GROUP = 16  # query heads per kv head of the single-token calls
 _BF16 = torch.bfloat16
 
@@ -62,7 +63,7 @@ def _shape4(t, name: str, want: str):
 
 
 def _counts(x, name: str, batch: int, dev, least: int, most: int):
-    """(device address or None, number for all) of per-sequence positions or lengths."""
+    """(device address or 0, number for all) of per-sequence positions or lengths."""
     if isinstance(x, torch.Tensor):
         if x.dtype is not torch.int32 or x.shape != (batch,) or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of {batch} entries, got {tuple(x.shape)} {x.dtype}")
@@ -72,7 +73,7 @@ def _counts(x, name: str, batch: int, dev, least: int, most: int):
     x = int(x)
     if not least <= x <= most:
         raise ValueError(f"{name} must be in [{least}, {most}], got {x}")
-    return None, x
+    return 0, x
 
 
 def _int32(x, name: str) -> int:
@@ -123,15 +124,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if not q.is_cuda:
         raise RuntimeError("kvm_b200 runs on CUDA tensors only (there is no CPU path)")
     qa, ka, va = _rows(q, "q", (B, Hq, T, D), dev), _rows(k, "k", (B, Hkv, S, D), dev), _rows(v, "v", (B, Hkv, S, D), dev)
-    lens = None
+    lens = 0
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor):
             raise ValueError(f"lengths must be an int32 tensor, got {type(lengths)}")
         lens, _ = _counts(lengths, "lengths", B, dev, 0, S)
     y = _output(out, q, (B, T, Hq * D))
-    args = _lib.KvmWindowPromptArgs(*qa[:4], *ka[:4], *va[:4], lens, y.data_ptr(), T, S, max(S, 1) if window is None else _int32(window, "window"),
-                                    _int32(sinks, "sinks"), B, Hq, Hkv, D, _scale(scale, D))
-    _call(dev, _lib.load().kvm_window_attention, C.addressof(args))
+    _call(dev, _lib.load().kvm_window_attention,
+          _pack_prompt(*qa[:4], *ka[:4], *va[:4], lens, y.data_ptr(), T, S, max(S, 1) if window is None else _int32(window, "window"),
+                       _int32(sinks, "sinks"), B, Hq, Hkv, D, _scale(scale, D)))
     return y
 
 
@@ -164,6 +165,8 @@ class WindowCache:
             self._k, self._v = (torch.zeros(shape, device=dev, dtype=_BF16) for _ in range(2))
             c.k, c.v = self._k.data_ptr(), self._v.data_ptr()
         self._addr = C.addressof(c)
+        self._like = torch.empty(0, device=dev, dtype=_BF16)
+        self._read_shape = (2, self.batch, self.n_kv_heads, self.sinks + self.window, self.head_dim)
         self._workspace_bytes: dict[int, int] = {}
 
     @property
@@ -187,16 +190,14 @@ class WindowCache:
         shape = (self.batch, self.n_kv_heads, T, self.head_dim)
         ka, va = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
         p, p_all = _counts(positions, "positions", self.batch, self.device, -1, 2**31 - 1 - T)
-        n, n_all = (None, T) if lengths is None else _counts(lengths, "lengths", self.batch, self.device, 0, T)
-        args = _lib.KvmWindowWriteArgs(self._addr, *ka[:4], *va[:4], p, n, T, p_all, n_all)
-        _call(self.device, _lib.load().kvm_window_cache_write, C.addressof(args))
+        n, n_all = (0, T) if lengths is None else _counts(lengths, "lengths", self.batch, self.device, 0, T)
+        _call(self.device, _lib.load().kvm_window_cache_write, _pack_write(self._addr, *ka[:4], *va[:4], p, n, T, p_all, n_all))
 
     def read(self, lengths) -> tuple[torch.Tensor, torch.Tensor]:
         """What the cache holds of sequences of ``lengths`` tokens, in order: (k, v) [B,Hkv,sinks+window,D], the first sinks
         tokens, then the last ``window`` ones; zeros behind the last token."""
         n, n_all = _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1)
-        kv = torch.empty((2, self.batch, self.n_kv_heads, self.sinks + self.window, self.head_dim), device=self.device, dtype=_BF16)
-        k, v = kv.unbind(0)
+        k, v = self._like.new_empty(self._read_shape).unbind(0)
         _call(self.device, _lib.load().kvm_window_cache_read, self._addr, n, n_all, k.data_ptr(), v.data_ptr())
         return k, v
 
@@ -212,15 +213,15 @@ class WindowCache:
         y = _output(out, q, (self.batch, 1, Hq * self.head_dim))
         # partial results: of this call alone (calls on two streams, or in two captured graphs, do not share them)
         ws = q.new_empty(need >> 1) if need else None
-        args = _lib.KvmWindowAttendArgs(self._addr, *qa[:4], *ka, *va, counts[0], y.data_ptr(), ws.data_ptr() if need else None, need, Hq,
-                                        counts[1], _scale(scale, self.head_dim))
-        _call(self.device, lib.kvm_window_attend, C.addressof(args))
+        _call(self.device, lib.kvm_window_attend,
+              _pack_attend(self._addr, *qa[:4], *ka, *va, counts[0], y.data_ptr(), ws.data_ptr() if need else 0, need, Hq, counts[1],
+                           _scale(scale, self.head_dim)))
         return y
 
     def attend(self, q: torch.Tensor, lengths, *, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """One query per sequence over the cached tokens: q [B,Hq,1,D], ``lengths`` the tokens of the sequences, the query's own
         among them.  Returns [B,1,Hq*D]; a sequence of no tokens gets zeros."""
-        none = (None, 0, 0, 0)
+        none = (0, 0, 0, 0)
         return self._attend(q, none, none, _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1), scale, out)
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions, *, scale: float | None = None,

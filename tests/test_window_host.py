@@ -111,3 +111,9 @@ def test_scales_beyond_the_range_are_refused():
     lib, c = _lib.load(), _cache()
     a = _lib.KvmWindowAttendArgs(C.addressof(c), 256, 128, 64, 64, None, 0, 0, 0, None, 0, 0, 0, None, 256, None, 0, 2, 4, 2.9e38)
     assert lib.kvm_window_attend(C.addressof(a), None) == 1 and "scale" in _err()
+
+
+@pytest.mark.parametrize("cls", [_lib.KvmWindowWriteArgs, _lib.KvmWindowAttendArgs, _lib.KvmWindowPromptArgs])
+def test_packed_blocks_are_what_the_structures_hold(cls):
+    values = [0.25 if t is C.c_float else 2**31 - 1 - i if t is C.c_int32 else 2**40 + i for i, (_, t) in enumerate(cls._fields_)]
+    assert _lib.packer(cls)(*values) == bytes(cls(*values))
