@@ -86,6 +86,8 @@ def _int32(x, name: str) -> int:
 def _output(out, like: torch.Tensor, shape) -> torch.Tensor:
     if out is None:
         return like.new_empty(shape)
+    if not isinstance(out, torch.Tensor) or (out.requires_grad and torch.is_grad_enabled()):
+        raise ValueError("out must be a tensor that needs no gradient")
     if out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous() or out.device != like.device or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned bf16 tensor {list(shape)} on {like.device}, got {list(out.shape)} {out.dtype}")
     return out
@@ -209,7 +211,8 @@ class WindowCache:
         if need is None:
             if Hq <= 0 or Hq % self.n_kv_heads or Hq // self.n_kv_heads > MAX_GROUP:
                 raise ValueError(f"{Hq} query heads over {self.n_kv_heads} kv heads: a multiple of them, at most {MAX_GROUP} each")
-            need = self._workspace_bytes[Hq] = lib.kvm_window_attend_workspace_bytes(self._addr, Hq)
+            with torch.cuda.device(self.device):
+                need = self._workspace_bytes[Hq] = lib.kvm_window_attend_workspace_bytes(self._addr, Hq)
         y = _output(out, q, (self.batch, 1, Hq * self.head_dim))
         # partial results: of this call alone (calls on two streams, or in two captured graphs, do not share them)
         ws = q.new_empty(need >> 1) if need else None

@@ -563,3 +563,14 @@ window.check_status()
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_outputs_that_cannot_be_written_are_refused():
+    from kvm_paper_b200 import window
+    q, k = (torch.zeros(2, h, 8, 64, device="cuda", dtype=torch.bfloat16) for h in (4, 2))
+    for out in (torch.zeros(2, 8, 256, device="cuda", dtype=torch.bfloat16, requires_grad=True), [0], torch.zeros(2, 8, 256, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            window.window_attention(q, k, k, window=4, out=out)
+    c = window.WindowCache(2, 2, 64, window=8)
+    with pytest.raises(ValueError):
+        c.attend(q[:, :, :1], 3, out=torch.zeros(2, 1, 256, device="cuda", dtype=torch.bfloat16, requires_grad=True))
