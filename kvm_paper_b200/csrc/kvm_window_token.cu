@@ -11,12 +11,12 @@
 // dimension and the query heads on N (8 or 16 columns).
 // 4 bits: the codes become f16 with one conversion instruction per two values.  q is scaled by a power of two per head into
 // f16's range.  A key group's scale multiplies the fp32 sum of its group; a value group's scale multiplies the weights, as
-// f16 relative to the largest power of two R in the scales seen so far (the output is rescaled when R rises, as with the
+// f16 relative to the largest power of two R in the group's scales so far (its outputs are rescaled when R rises, as with the
 // softmax maximum).  Weights go up to 2^8 and scales to 2^7, so that the product uses f16 to its top: scales down to 2^-25 R and
 // weights down to 2^-22 of the largest keep all their bits, smaller ones an error of 2^-31 R and 2^-33 of the largest.
 // The new token: the CTA that reads the chunk with its row patches the stage and writes the row to memory.
 //
-// Measured: 4 bits, 64 x 4 kv rows of 16384 x 128 129 us (4.7 TB/s of codes and scales), one sequence of 262144 x 8 kv rows 68 us
+// Measured: 4 bits, 64 x 4 kv rows of 16384 x 128 130 us (4.6 TB/s of codes and scales), one sequence of 262144 x 8 kv rows 69 us
 // (4.4 TB/s): half of the ALU's and of the issue slots go into unpacking codes, the rest is the latency of a warp's dependent
 // steps, for which the registers leave room for eight warps.  16 bits, 64 x 4 kv rows of 4100 x 128 80 us (6.7 TB/s): memory.  A
 // few hundred tokens: 5 to 7 us, launch and two round trips to memory.
@@ -86,6 +86,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {  // (2^-23; of 0: infinity)
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -144,7 +149,7 @@ struct Place {
   int b, h, c, n_chunks;  // sequence, kv head, chunk of the kv row, chunks of the kv row
 };
 
-// Partial result of a kv row that a CTA's range cuts: [head][m, l, acc[D]].
+// Partial result of a kv row that a CTA's range cuts: [head][m, l, output[D]], the output divided by l.
 __host__ __device__ inline size_t partial_floats(int D, int G) { return (size_t)G * (D + 2); }
 
 // The split of the list, the same in both kernels.  whole_rows: ranges end between kv rows.
@@ -380,7 +385,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
     float qs[NH][2];                 // softmax scale (log2) of this thread's heads 2t, 2t + 1
     float o[NH][D / 16][4];          // output: channels x heads
     float m[NH][2], l[NH][2];
-    unsigned r_bits = 0;             // 4 bits: R, as the exponent field of a bf16 pattern (0: none yet)
+    unsigned r_bits = 0;             // 4 bits: R of group lane % NG, as the exponent field of a bf16 pattern (0: none yet)
 #pragma unroll
     for (int hb = 0; hb < NH; ++hb) {
       m[hb][0] = m[hb][1] = kLowest;
@@ -501,7 +506,6 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
       // groups u0 .. u0 + N - 1 of this warp's rows
       auto groups = [&](auto count, int u0) {
         constexpr int N = decltype(count)::value;
-        float r_alpha = 1.f;
         if (BITS == 4) {  // the value scales relative to R as f16, each lane a pair of rows' of a group
           uint32_t x[N], top2 = 0;
 #pragma unroll
@@ -509,11 +513,20 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             x[u] = lane < 8 * NG ? *reinterpret_cast<const uint32_t*>(st + (warp + (u0 + u) * kMathWarps) * Block4<D>::kBytes + Block4<D>::kValueScales + lane * 4) : 0u;
             top2 = __vmaxs2(top2, x[u]);  // (the NaN of a scale is negative: it reaches its own group only)
           }
-          // the exponent of the largest of them
-          const unsigned top = __reduce_max_sync(kAll, max(top2 & 0xffffu, top2 >> 16)) & 0x7f80u;
-          if (top > r_bits) {
-            r_alpha = r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
-            r_bits = top;
+          unsigned top = max(top2 & 0xffffu, top2 >> 16) & 0x7f80u;
+          if (__any_sync(kAll, top > r_bits)) {  // a group's R rises, to the exponent of the largest of its scales
+#pragma unroll
+            for (int d = NG; d < 8 * NG; d <<= 1) top = max(top, __shfl_xor_sync(kAll, top, d));
+            const float down = top <= r_bits ? 1.f : r_bits ? __uint_as_float((unsigned)max(127 + (int)(r_bits >> 7) - (int)(top >> 7), 0) << 23) : 0.f;
+            r_bits = max(r_bits, top);
+#pragma unroll
+            for (int k2 = 0; k2 < D / 16; ++k2) {
+              const float a = __shfl_sync(kAll, down, k2 >> 1);
+#pragma unroll
+              for (int hb = 0; hb < NH; ++hb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[hb][k2][e] *= a;
+            }
           }
           // (a scale is below 2 R here, a weight at most 2^8: with 2^6 / R, f16 just holds the product)
           const unsigned e_r = r_bits >> 7;
@@ -587,8 +600,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
         }
 
-        // ---- weights up to 2^kTop: the reference m is that much below the running maximum (4 bits: f16 holds 2^-24 .. 2^15)
-        constexpr float kTop = BITS == 4 ? 8.f : 0.f;
+        // ---- weights up to 2^kTop: the reference m is that much below the running maximum.  4 bits: f16 holds 2^-24 .. 2^15.
+        // 16 bits: small enough that 2^24 of the largest bf16 numbers stay inside fp32's range.
+        constexpr float kTop = BITS == 4 ? 8.f : -24.f;
         float alpha[NH][2];
 #pragma unroll
         for (int hb = 0; hb < NH; ++hb) {
@@ -617,7 +631,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         for (int hb = 0; hb < NH; ++hb) {
           l[hb][0] *= alpha[hb][0];
           l[hb][1] *= alpha[hb][1];
-          const float2 a = make_float2(alpha[hb][0] * r_alpha, alpha[hb][1] * r_alpha);
+          const float2 a = make_float2(alpha[hb][0], alpha[hb][1]);
 #pragma unroll
           for (int e = 0; e < D / 16; ++e) {
             const float2 x = __fmul2_rn(make_float2(o[hb][e][0], o[hb][e][1]), a), y = __fmul2_rn(make_float2(o[hb][e][2], o[hb][e][3]), a);
@@ -721,6 +735,13 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
     }
 
     // ---- join the warps
+    // (outputs are divided by their sums at once, so that none passes fp32's range on the way)
+    float up[NG];  // what the outputs of a group are to be multiplied by
+#pragma unroll
+    for (int n2 = 0; n2 < NG; ++n2) {
+      const unsigned r = __shfl_sync(kAll, r_bits, n2);
+      up[n2] = BITS == 4 ? __uint_as_float(r << 16) * __uint_as_float((127u - min(r >> 7, kScaleUp)) << 23) : 1.f;
+    }
 #pragma unroll
     for (int hb = 0; hb < NH; ++hb) {
 #pragma unroll
@@ -729,6 +750,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         x += __shfl_xor_sync(kAll, x, 4);
         x += __shfl_xor_sync(kAll, x, 8);
         x += __shfl_xor_sync(kAll, x, 16);
+        const float inv = x == 0.f ? 0.f : rcp(x);
         const int head = hb * 8 + 2 * t + e;
         if (g == 0) {
           wmax[warp * 16 + head] = m[hb][e];
@@ -736,13 +758,12 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         }
         if (head < G) {
           float* dst = ored + ((size_t)warp * G + head) * D;
-          const float up = BITS == 4 ? __uint_as_float(r_bits << 16) * __uint_as_float((127u - min(r_bits >> 7, kScaleUp)) << 23) : 1.f;
 #pragma unroll
           for (int k2 = 0; k2 < D / 16; ++k2) {
             // 4 bits: channels 32 (k2/2) + 4 g + 2 (k2%2) + {0, 1};  16 bits: 64 (k2/4) + 8 g + 2 (k2%4) + {0, 1}, and for
             // D = 32: 4 g + 2 k2 + {0, 1}
             const int ch = BITS == 4 || D == 32 ? (k2 >> 1) * 32 + 4 * g + 2 * (k2 & 1) : (k2 >> 2) * 64 + 8 * g + 2 * (k2 & 3);
-            *reinterpret_cast<float2*>(dst + ch) = make_float2(o[hb][k2][e] * up, o[hb][k2][e + 2] * up);
+            *reinterpret_cast<float2*>(dst + ch) = make_float2(o[hb][k2][e] * inv * up[k2 >> 1], o[hb][k2][e + 2] * inv * up[k2 >> 1]);
           }
         }
       }
@@ -755,17 +776,21 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
       float mx = kLowest;
 #pragma unroll
       for (int w = 0; w < kMathWarps; ++w) mx = fmaxf(mx, wmax[w * 16 + head]);
-      float sum = 0.f, a0 = 0.f, a1 = 0.f;
+      float f[kMathWarps], sum = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
       for (int w = 0; w < kMathWarps; ++w) {
-        const float f = ex2(wmax[w * 16 + head] - mx);
+        f[w] = ex2(wmax[w * 16 + head] - mx) * wsum[w * 16 + head];
+        sum += f[w];
+      }
+      const float inv = rcp(sum);  // (no score above -inf: 0 x inf)
+#pragma unroll
+      for (int w = 0; w < kMathWarps; ++w) {
         const float2 y = *reinterpret_cast<const float2*>(ored + ((size_t)w * G + head) * D + ch);
-        sum = fmaf(wsum[w * 16 + head], f, sum);
-        a0 = fmaf(y.x, f, a0);
-        a1 = fmaf(y.y, f, a1);
+        a0 = fmaf(y.x, f[w] * inv, a0);
+        a1 = fmaf(y.y, f[w] * inv, a1);
       }
       if (whole) {
-        *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + pl.b) * Hq + pl.h * G + head) * D + ch) = pack_bf16(a0 / sum, a1 / sum);
+        *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + pl.b) * Hq + pl.h * G + head) * D + ch) = pack_bf16(a0, a1);
       } else {
         float* dst = partial + ((size_t)blockIdx.x * 2 + slot) * partial_floats(D, G) + (size_t)head * (D + 2);
         *reinterpret_cast<float2*>(dst + 2 + ch) = make_float2(a0, a1);
@@ -830,9 +855,9 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
   float sum = 0.f;
   for (int i = tid; i < n; i += 256) {
     const float2 ml = *reinterpret_cast<const float2*>(src(i));
-    const float f = ex2(ml.x - mx);
+    const float f = ex2(ml.x - mx) * ml.y;
     weight[i] = f;
-    sum = fmaf(f, ml.y, sum);
+    sum += f;
   }
   sum = warp_sum(sum);
   if ((tid & 31) == 0) red[1][tid >> 5] = sum;
@@ -840,13 +865,15 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
   sum = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) sum += red[1][w];
+  const float inv = rcp(sum);
   const int col = tid % COLS, grp = tid / COLS;
   float2 acc = make_float2(0.f, 0.f);
 #pragma unroll 8
   for (int i = grp; i < n; i += GROUPS) {
     const float2 x = *reinterpret_cast<const float2*>(src(i) + 2 + col * 2);
-    acc.x = fmaf(weight[i], x.x, acc.x);
-    acc.y = fmaf(weight[i], x.y, acc.y);
+    const float f = weight[i] * inv;
+    acc.x = fmaf(f, x.x, acc.x);
+    acc.y = fmaf(f, x.y, acc.y);
   }
   part[tid] = acc;
   __syncthreads();
@@ -855,7 +882,7 @@ kvm_window_join_kernel(WindowDev W, int G, SeqInts lens, int extra, int chunk, i
       acc.x += part[i * COLS + col].x;
       acc.y += part[i * COLS + col].y;
     }
-    *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + b) * Hkv * G + h * G + head) * D + col * 2) = pack_bf16(acc.x / sum, acc.y / sum);
+    *reinterpret_cast<uint32_t*>(out + ((size_t)(b0 + b) * Hkv * G + h * G + head) * D + col * 2) = pack_bf16(acc.x, acc.y);
   }
 }
 

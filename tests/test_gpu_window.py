@@ -574,3 +574,24 @@ def test_outputs_that_cannot_be_written_are_refused():
     c = window.WindowCache(2, 2, 64, window=8)
     with pytest.raises(ValueError):
         c.attend(q[:, :, :1], 3, out=torch.zeros(2, 1, 256, device="cuda", dtype=torch.bfloat16, requires_grad=True))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("n", [40, 1500, 30000])
+def test_token_values_near_the_largest_number(bits, n):
+    """Sums of weights that are not normalised yet would pass the range of fp32; the output does not."""
+    from kvm_paper_b200 import window
+    g = _gen(41 + n)
+    k, v = wh.heads_data(g, 2, 1, n, 64), wh.heads_data(g, 2, 1, n, 64)
+    v[0] = 3e38
+    v[0, :, :, 32:40] = -3e38
+    v[1, :, :, :32] *= 5e37
+    q = wh.heads_data(g, 2, 3, 1, 64)
+    c = window.WindowCache(2, 1, 64, window=n, bits=bits)
+    c.write(k, v, 0)
+    got = c.attend(q, n).view(2, 3, 64)
+    assert bool(torch.isfinite(got).all())
+    hk, hv = (wh.quantised(k), wh.quantised(v)) if bits == 4 else (k.double(), v.double())
+    for b in range(2):
+        want, mag = wh.attend(q[b], hk[b], hv[b], torch.ones(1, n, device="cuda", dtype=torch.bool), 64 ** -0.5)
+        wh.assert_near(got[b], want[:, 0], mag[:, 0], bits)
