@@ -465,8 +465,8 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
       }
-      const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-      poison |= !(tmax < INFINITY);  // NaN or +inf among the scores: the row is NaN
+      const float tmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
+      poison |= !(tmax < INFINITY);  // NaN or +inf among the scores: the row is NaN (the polynomial below does not carry a NaN on)
       const bool need = tmax > m_run + kRescale || (m_run == -INFINITY && tmax > -INFINITY);
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? tmax : m_run;
