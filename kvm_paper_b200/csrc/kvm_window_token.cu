@@ -782,7 +782,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         f[w] = ex2(wmax[w * 16 + head] - mx) * wsum[w * 16 + head];
         sum += f[w];
       }
-      const float inv = rcp(sum);  // (no score above -inf: 0 x inf)
+      // (no score above -inf: NaN, 0 x inf, if that is all of the kv row; a share of one that is cut adds zeros)
+      const float inv = sum == 0.f && !whole ? 0.f : rcp(sum);
 #pragma unroll
       for (int w = 0; w < kMathWarps; ++w) {
         const float2 y = *reinterpret_cast<const float2*>(ored + ((size_t)w * G + head) * D + ch);

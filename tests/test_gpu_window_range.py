@@ -33,3 +33,31 @@ def test_prompt_a_key_that_is_nan_reaches_every_row_that_sees_it(dim, window_, s
     want, mag = wh.prompt(q, k, v, window_, sinks)
     assert int(torch.isnan(want).sum()) > 300 * H * dim
     wh.assert_near(got, want, mag)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_token_a_share_without_a_score_adds_nothing(bits):
+    """Long rows are cut between CTAs: shares whose every score is -inf (16 bits: infinities among the keys; 4 bits: sums beyond
+    fp32, of which the definition's weights are zero as well) beside shares with scores, and rows with none at all."""
+    from kvm_paper_b200 import window
+    g = _gen(51)
+    n, dim = 40000, 64
+    q = wh.heads_data(g, 1, 4, 1, dim).abs() + 0.25
+    v = wh.heads_data(g, 1, 2, n, dim)
+    k = wh.heads_data(g, 1, 2, n, dim)
+    for head, rows in ((0, slice(0, 21000)), (1, slice(15000, n))):
+        k[0, head, rows] = -3e38
+        if bits == 16:
+            k[0, head, rows, 7] = -math.inf
+    c = window.WindowCache(1, 2, dim, window=n, bits=bits)
+    c.write(k, v, 0)
+    got = c.attend(q, n).view(4, dim)
+    hk, hv = (wh.quantised(k), wh.quantised(v)) if bits == 4 else (k.double(), v.double())
+    want, mag = wh.attend(q[0], hk[0], hv[0], torch.ones(1, n, device="cuda", dtype=torch.bool), dim ** -0.5)
+    assert bool(torch.isfinite(want).all())
+    wh.assert_near(got, want[:, 0], mag[:, 0], bits)
+    if bits == 16:
+        k[0, 0, :, 7] = -math.inf
+        c.write(k, v, 0)
+        got = c.attend(q, n).view(2, 2, dim)
+        assert bool(torch.isnan(got[0]).all()) and torch.equal(got[1].double(), got[1].double().nan_to_num(nan=9.0))
