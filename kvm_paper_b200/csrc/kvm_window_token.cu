@@ -35,7 +35,7 @@ constexpr int kMaxStages = 8;
 constexpr int kBox = 128;                     // rows per TMA box (16 bits; the end of a cache comes in boxes of 16)
 constexpr int kSmemPerSm = 228 * 1024;        // of which every CTA takes 1 KB more than it asks for
 constexpr int kMaxBatch = 1024;               // sequences per launch
-constexpr float kLowest = -3e38f;             // reference of the weights before the first score
+constexpr float kLowest = -3.402823466e38f;   // reference of the weights before the first score: no finite one is below it
 constexpr unsigned kScaleUp = 6;              // see R below
 
 // How a variant works.  4 bits: bound by the math warps (conversions and fixed latencies), which is why a warp takes T = 4 groups of
@@ -600,8 +600,20 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           }
         }
 
+        // ---- in units of log2, each rounded as a number of its own: as a fused product and difference below, a score of 2^31
+        // would lie further from its own rounded value than a weight reaches.  (Before the mask: a scale may be as small as to
+        // count as 0, and 0 x inf is NaN.)
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int hb = 0; hb < NH; ++hb) {
+            const float2 f = make_float2(qs[hb][0], qs[hb][1]);
+            const float2 x = __fmul2_rn(make_float2(sc[u][hb][0], sc[u][hb][1]), f), y = __fmul2_rn(make_float2(sc[u][hb][2], sc[u][hb][3]), f);
+            sc[u][hb][0] = x.x; sc[u][hb][1] = x.y; sc[u][hb][2] = y.x; sc[u][hb][3] = y.y;
+          }
         // ---- weights up to 2^kTop: the reference m is that much below the running maximum.  4 bits: f16 holds 2^-24 .. 2^15.
-        // 16 bits: small enough that 2^24 of the largest bf16 numbers stay inside fp32's range.
+        // 16 bits: small enough that 2^24 of the largest bf16 numbers stay inside fp32's range.  Of scores beyond 2^20 m is the
+        // maximum itself, which kTop could round away from by more than it says.
         constexpr float kTop = BITS == 4 ? 8.f : -24.f;
         float alpha[NH][2];
 #pragma unroll
@@ -620,10 +632,10 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             for (int u = 1; u < N; ++u) x = fmaxf(x, fmaxf(sc[u][hb][e], sc[u][hb][e + 2]));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(kAll, x, 16)) * qs[hb][e];  // (positive)
-            const bool up = x > m[hb][e] + kTop;
-            alpha[hb][e] = up ? ex2(m[hb][e] - (x - kTop)) : 1.f;
-            m[hb][e] = up ? x - kTop : m[hb][e];
+            x = fmaxf(x, __shfl_xor_sync(kAll, x, 16));
+            const float top = fmaxf(m[hb][e], fabsf(x) < 0x1p20f ? x - kTop : x);
+            alpha[hb][e] = ex2(m[hb][e] - top);
+            m[hb][e] = top;
           }
         }
         // (always: the FMA pipe is idle, and without a branch the rest of the chunk mixes with it)
@@ -645,7 +657,11 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
           for (int hb = 0; hb < NH; ++hb) {
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(sc[u][hb][e], qs[hb][e & 1], -m[hb][e & 1]));
+            for (int e = 0; e < 4; e += 2) {
+              const float2 x = __fadd2_rn(make_float2(sc[u][hb][e], sc[u][hb][e + 1]), make_float2(-m[hb][0], -m[hb][1]));
+              p[e] = ex2(x.x);
+              p[e + 1] = ex2(x.y);
+            }
             l[hb][0] += p[0] + p[2];
             l[hb][1] += p[1] + p[3];
             pb[u][hb][0] = movmatrix_trans(BITS == 4 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));

@@ -61,3 +61,51 @@ def test_token_a_share_without_a_score_adds_nothing(bits):
         c.write(k, v, 0)
         got = c.attend(q, n).view(2, 2, dim)
         assert bool(torch.isnan(got[0]).all()) and torch.equal(got[1].double(), got[1].double().nan_to_num(nan=9.0))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("dim,group", [(128, 1), (64, 9), (32, 2)])
+def test_token_queries_of_zeros_with_the_smallest_scales(bits, dim, group):
+    """All scores 0: the mean of the values, whatever the scale, over rows that are seen in part, too."""
+    from kvm_paper_b200 import window
+    g = _gen(53)
+    n = [1, 17, 100, 333]
+    k, v = wh.heads_data(g, 4, 1, 333, dim), wh.heads_data(g, 4, 1, 333, dim)
+    c = window.WindowCache(4, 1, dim, window=290, sinks=3, bits=bits)
+    c.write(k, v, 0, lengths=_ints(n))
+    ref = wh.Cache(4, 1, dim, 290, 3, bits)
+    q = torch.zeros(4, group, 1, dim, device="cuda", dtype=torch.bfloat16)
+    q[:, -1] = 1e-38
+    for scale in (1e-37, 1e-20, 1e-6, 1.0):
+        got = c.attend(q, _ints(n), scale=scale)
+        for b in range(4):
+            ref.write(b, k[b, :, :n[b]], v[b, :, :n[b]], 0)
+            want, mag = ref.attend(b, q[b], n[b], scale)
+            wh.assert_near(got[b, 0], want.flatten(), mag.flatten(), bits, f"scale {scale}, {n[b]} tokens")
+
+
+def _one_hot(up, sign, heads, rows, dim):
+    """Keys of one channel, 97 levels from 2^up on, the same again every 97 keys: scores of any size, far apart or alike."""
+    k = torch.zeros(1, heads, rows, dim, device="cuda", dtype=torch.bfloat16)
+    k[..., 5] = ((1 + torch.arange(rows, device="cuda") % 97 / 128) * 2.0 ** up * sign).bfloat16()
+    return k
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("up", [10, 13, 14, 15, 16, 17, 18, 19, 20, 30, 50, 60])
+def test_token_scores_of_any_size(bits, sign, up):
+    """Scores of 2^21 to 2^121, all of them finite: the keys with the largest one share the whole weight."""
+    from kvm_paper_b200 import window
+    g = _gen(60 + up)
+    for dim, group, n in ((64, 3, 500), (128, 9, 900), (32, 8, 9000)):
+        k, v = _one_hot(up, sign, 1, n, dim), wh.heads_data(g, 1, 1, n, dim)
+        q = torch.zeros(1, group, 1, dim, device="cuda", dtype=torch.bfloat16)
+        q[..., 5] = (1.3 + torch.arange(group, device="cuda").view(1, -1, 1) / 16) * 2.0 ** up
+        c = window.WindowCache(1, 1, dim, window=n, bits=bits)
+        c.write(k, v, 0)
+        for scale in (None, 1.0):
+            got = c.attend(q, n, scale=scale).view(group, dim)
+            hk, hv = (wh.quantised(k), wh.quantised(v)) if bits == 4 else (k.double(), v.double())
+            want, mag = wh.attend(q[0], hk[0], hv[0], torch.ones(1, n, device="cuda", dtype=torch.bool), scale or dim ** -0.5)
+            wh.assert_near(got, want[:, 0], mag[:, 0], bits)
