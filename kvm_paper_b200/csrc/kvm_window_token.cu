@@ -382,7 +382,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
     int plain_from, plain_to;  // chunks that are seen whole
     seen.whole_chunks(CH, plain_from, plain_to);
     uint32_t qf[NH][D / 16][2];      // queries as B fragments
-    float qs[NH][2];                 // softmax scale (log2) of this thread's heads 2t, 2t + 1
+    float qs[NH][2], qd[NH][2];      // of this thread's heads 2t, 2t + 1: what scores are multiplied by, and 4 bits: a group's sums
     float o[NH][D / 16][4];          // output: channels x heads
     float m[NH][2], l[NH][2];
     unsigned r_bits = 0;             // 4 bits: R of group lane % NG, as the exponent field of a bf16 pattern (0: none yet)
@@ -436,9 +436,15 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
                 const float2 f = unpack_bf16(x[n2][e2]);
                 qf[hb][n2 * 2 + (e2 >> 1)][e2 & 1] = pack_f16(f.x * up, f.y * up);
               }
-            // this thread's scores are of heads 2t, 2t + 1: their factors lie in lanes 8t, 8t + 4
-            qs[hb][0] = __shfl_sync(kAll, down, 8 * t) * scale_log2;
-            qs[hb][1] = __shfl_sync(kAll, down, 8 * t + 4) * scale_log2;
+            // this thread's scores are of heads 2t, 2t + 1: their factors lie in lanes 8t, 8t + 4.  The part of a factor that
+            // makes sums smaller goes to a group's sums ahead of the keys' scale, the part that makes them larger to the
+            // scores: neither passes fp32's range unless the score does.
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              const float f = __shfl_sync(kAll, down, 8 * t + 4 * e2) * scale_log2;
+              qd[hb][e2] = fminf(f, 1.f);
+              qs[hb][e2] = fminf(fmaxf(f, 1.f), 3e38f);
+            }
           } else {
             constexpr int PER = D >= 64 ? 4 : 2;  // k-steps per 64 (32) channels; a thread's channels are contiguous
 #pragma unroll
@@ -571,10 +577,14 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
                 float acc[4];
                 mma_f16_zero(acc, a[0], c[0], a[1], c[1], qf[hb][n2 * 2][0], qf[hb][n2 * 2][1]);
                 mma_f16(acc, a[2], c[2], a[3], c[3], qf[hb][n2 * 2 + 1][0], qf[hb][n2 * 2 + 1][1]);
-                sc[u][hb][0] = fmaf(ks[0][n2], acc[0], sc[u][hb][0]);
-                sc[u][hb][1] = fmaf(ks[0][n2], acc[1], sc[u][hb][1]);
-                sc[u][hb][2] = fmaf(ks[1][n2], acc[2], sc[u][hb][2]);
-                sc[u][hb][3] = fmaf(ks[1][n2], acc[3], sc[u][hb][3]);
+                const float2 f = make_float2(qd[hb][0], qd[hb][1]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(acc[2 * r], acc[2 * r + 1]), f), make_float2(ks[r][n2], ks[r][n2]),
+                                              make_float2(sc[u][hb][2 * r], sc[u][hb][2 * r + 1]));
+                  sc[u][hb][2 * r] = y.x;
+                  sc[u][hb][2 * r + 1] = y.y;
+                }
               }
             }
           } else {

@@ -109,3 +109,42 @@ def test_token_scores_of_any_size(bits, sign, up):
             hk, hv = (wh.quantised(k), wh.quantised(v)) if bits == 4 else (k.double(), v.double())
             want, mag = wh.attend(q[0], hk[0], hv[0], torch.ones(1, n, device="cuda", dtype=torch.bool), scale or dim ** -0.5)
             wh.assert_near(got, want[:, 0], mag[:, 0], bits)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("up", [-112, -60, 60, 112])
+def test_token_queries_and_keys_of_opposite_size(bits, up):
+    """Scores as in any other call, of queries near one end of the range and keys near the other."""
+    from kvm_paper_b200 import window
+    g = _gen(54)
+    for dim, group, n in ((128, 4, 300), (64, 16, 3000), (32, 1, 70)):
+        k, v, q = wh.heads_data(g, 2, 1, n, dim), wh.heads_data(g, 2, 1, n, dim), wh.heads_data(g, 2, group, 1, dim)
+        k, q = (k.float() * 2.0 ** up).bfloat16(), (q.float() * 2.0 ** -up).bfloat16()
+        c = window.WindowCache(2, 1, dim, window=n, bits=bits)
+        c.write(k, v, 0)
+        got = c.attend(q, n).view(2, group, dim)
+        hk, hv = (wh.quantised(k), wh.quantised(v)) if bits == 4 else (k.double(), v.double())
+        for b in range(2):
+            want, mag = wh.attend(q[b], hk[b], hv[b], torch.ones(1, n, device="cuda", dtype=torch.bool), dim ** -0.5)
+            wh.assert_near(got[b], want[:, 0], mag[:, 0], bits)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_token_keys_near_the_largest_number(bits):
+    """Scores of up to 2^125, all of them finite: the key with the largest one takes the whole weight."""
+    from kvm_paper_b200 import window
+    g = _gen(55)
+    dim, n = 64, 500
+    k, v = torch.zeros(1, 1, n, dim, device="cuda", dtype=torch.bfloat16), wh.heads_data(g, 1, 1, n, dim)
+    best = [7, 213, 499, 64]
+    for channel, i in enumerate(best):
+        k[0, 0, :, 16 * channel] = (torch.arange(n, device="cuda") % 97 * 1e35).bfloat16()
+        k[0, 0, i, 16 * channel] = 3.2e37  # (the largest of its row's group: held exactly or nearly)
+    q = torch.zeros(1, 4, 1, dim, device="cuda", dtype=torch.bfloat16)
+    for head in range(4):
+        q[0, head, 0, 16 * head] = 1.0
+    c = window.WindowCache(1, 1, dim, window=n, bits=bits)
+    c.write(k, v, 0)
+    got = c.attend(q, n).view(4, dim)
+    held = c.read(n)[1][0, 0]
+    assert torch.equal(got, held[best])
