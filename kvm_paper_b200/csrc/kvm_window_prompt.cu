@@ -165,18 +165,20 @@ __device__ __forceinline__ float fma_sat(float a, float b, float c) {  // clampe
   asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for two x in [-120, 8], given as y = (x + 120) / 128 (clamping to [0, 1] has clamped x).  Range reduction to the nearest
-// integer and a polynomial of degree 3 on [-1/2, 1/2], minimax in the relative error by Remez exchange: 7.5e-5, a
-// twenty-fifth of the bf16 rounding that follows.  On the FMA pipes: the special-function unit makes 16 exponentials per
-// clock and SM, and both query tiles' softmaxes want 128 x 128 each for every 2048 clocks of the tensor core.
+// 2^x for two x, given as y = (x + 127) / 256 clamped to [0, 1]: x <= -127 gives exactly 0, as below the smallest number.
+// Range reduction to the nearest integer and a polynomial 1 + f (a + b f + c f^2) on [-1/2, 1/2], minimax in the relative error by
+// linear programming: 1.07e-4, an eighteenth of the bf16 rounding that follows.  (With a constant term of its own it would be
+// 7.5e-5, but 2^-127 no longer the pattern of 0: just below 1 it wraps around to a negative number.)  On the FMA pipes: the
+// special-function unit makes 16 exponentials per clock and SM, and both query tiles' softmaxes want 128 x 128 each for every
+// 2048 clocks of the tensor core.
 __device__ __forceinline__ float2 ex2_fma(float2 y) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, which stands in the low bits
-  const float2 t = __ffma2_rn(y, make_float2(128.f, 128.f), make_float2(kMagic - 120.f, kMagic - 120.f));
-  const float2 n = __fadd2_rn(t, make_float2(120.f - kMagic, 120.f - kMagic));  // the integer + 120
-  const float2 f = __ffma2_rn(y, make_float2(128.f, 128.f), make_float2(-n.x, -n.y));
-  float2 p = __ffma2_rn(f, make_float2(0.0551716685295105f, 0.0551716685295105f), make_float2(0.2426111251115799f, 0.2426111251115799f));
-  p = __ffma2_rn(f, p, make_float2(0.6932609677314758f, 0.6932609677314758f));
-  p = __ffma2_rn(f, p, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  const float2 t = __ffma2_rn(y, make_float2(256.f, 256.f), make_float2(kMagic - 127.f, kMagic - 127.f));
+  const float2 n = __fadd2_rn(t, make_float2(127.f - kMagic, 127.f - kMagic));  // the integer + 127
+  const float2 f = __ffma2_rn(y, make_float2(256.f, 256.f), make_float2(-n.x, -n.y));
+  float2 p = __ffma2_rn(f, make_float2(0.05500893294811249f, 0.05500893294811249f), make_float2(0.2422109693288803f, 0.2422109693288803f));
+  p = __ffma2_rn(f, p, make_float2(0.6932829022407532f, 0.6932829022407532f));
+  p = __ffma2_rn(f, p, make_float2(1.f, 1.f));
   return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
@@ -496,11 +498,10 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
         }
         tc::fence_proxy_async();
       }
-      // weights; where every key is seen, some by polynomial (a masked weight has to be 0, which the polynomial's range
-      // does not hold)
+      // weights; where every key is seen, some by polynomial
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
-      const float sc128 = sc * (1.f / 128.f), nm128 = (neg_m + 120.f) * (1.f / 128.f);
+      const float sc256 = sc * (1.f / 256.f), nm256 = (neg_m + 127.f) * (1.f / 256.f);
       float2 ls = make_float2(0.f, 0.f);
       auto weights = [&](auto poly) {
 #pragma unroll
@@ -513,7 +514,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
               const float s0 = __uint_as_float(sr[c][e * 2]), s1 = __uint_as_float(sr[c][e * 2 + 1]);
               float2 w;
               if (decltype(poly)::value && (e * kPoly) / 16 != ((e + 1) * kPoly) / 16) {  // (spread evenly)
-                w = ex2_fma(make_float2(fma_sat(s0, sc128, nm128), fma_sat(s1, sc128, nm128)));
+                w = ex2_fma(make_float2(fma_sat(s0, sc256, nm256), fma_sat(s1, sc256, nm256)));
               } else {
                 const float2 z = __ffma2_rn(make_float2(s0, s1), sc2, nm2);
                 w = make_float2(ex2(z.x), ex2(z.y));

@@ -148,3 +148,26 @@ def test_token_keys_near_the_largest_number(bits):
     got = c.attend(q, n).view(4, dim)
     held = c.read(n)[1][0, 0]
     assert torch.equal(got, held[best])
+
+
+@pytest.mark.parametrize("dim", [128, 64])
+@pytest.mark.parametrize("far", [-200.0, -1000.0, -math.inf])
+def test_prompt_values_far_below_the_maximum_weigh_nothing(dim, far):
+    """Keys whose weight is below the smallest number hold values near the largest one, in every place of a tile that is seen
+    whole: 2^-200 * 2^127 and less, 2^-24 at the most for all of them."""
+    from kvm_paper_b200 import window
+    g = _gen(52)
+    H, T = 8, 400
+    q, k, v = (wh.heads_data(g, 1, H, T, dim, scale=s) for s in (1.0, 1.0, 1.0))
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    for h in range(H):  # every eighth key: scores in units of log2
+        k[0, h, h::8, 0] = far * math.log(2) * dim ** 0.5 if far > -math.inf else -math.inf
+        v[0, h, h::8] = 3e38
+    q, k, v = (t[:, :, 1:] if h == 0 else t for h, t in enumerate((q, k, v)))
+    got = window.window_attention(q, k, v, window=None).view(1, T - 1, H, dim)
+    want, mag = wh.prompt(q, k, v, None, 0)
+    # (head 0's first queries may see nothing but such keys: from query 8 on every row has another one)
+    want, mag, got = want[:, 8:], mag[:, 8:], got[:, 8:]
+    assert float(want.abs().max()) < 10
+    tol = (2 * wh.U_BF16 + 2.0 ** -8) * mag + 2.0 ** -20  # scores up to 2^10: as in the test of scores far apart
+    assert bool(((got.double() - want).abs() <= tol).all())
