@@ -617,9 +617,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
         for (int u = 0; u < N; ++u)
 #pragma unroll
           for (int hb = 0; hb < NH; ++hb) {
-            const float2 f = make_float2(qs[hb][0], qs[hb][1]);
-            const float2 x = __fmul2_rn(make_float2(sc[u][hb][0], sc[u][hb][1]), f), y = __fmul2_rn(make_float2(sc[u][hb][2], sc[u][hb][3]), f);
-            sc[u][hb][0] = x.x; sc[u][hb][1] = x.y; sc[u][hb][2] = y.x; sc[u][hb][3] = y.y;
+            // (scalar products: a packed one and a sum may be made one fused operation, even with the rounding named)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[u][hb][e] = __fmul_rn(sc[u][hb][e], qs[hb][e & 1]);
           }
         // ---- weights up to 2^kTop: the reference m is that much below the running maximum.  4 bits: f16 holds 2^-24 .. 2^15.
         // 16 bits: small enough that 2^24 of the largest bf16 numbers stay inside fp32's range.  Of scores beyond 2^20 m is the
