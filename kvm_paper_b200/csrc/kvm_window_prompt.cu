@@ -15,7 +15,7 @@
 //                          (fp32), P as bf16; behind the last tile O / l to global memory.
 // Infinities and NaN in values that a row does not see: a masked weight is 0, and 0 x inf would reach the row through the
 // product.  Value rows behind a sequence's length are cleared in shared memory; for any other, a row whose sum is finite
-// but whose output is not is settled by its thread from the keys that it sees (redo_columns).
+// but whose output is not is marked, and formed again from the keys that it sees when its warp's last tile is done (revisit).
 // Every wait is bounded; one that runs out sets the status word, and the CTA leaves through its common exit.
 //
 // Measured (32 / 8 heads x 128, 8192 queries over all earlier tokens): 461 us, 1190 TFLOP/s; 2 x 32768 queries, 16 heads x 128,
@@ -135,11 +135,10 @@ struct Item {
 };
 
 // Bounded wait without pauses of its own between the tries: the roles hand tiles to each other several times per microsecond,
-// and a pause that overshoots is on the path of both.  What is waited for comes within microseconds, but for a softmax warp that
-// looks through its rows' values again (redo_columns: up to 1.1 s behind 65536 keys).  A try that fails has waited for about
-// 2700 clocks: 2^26 of them are some 100 s.
+// and a pause that overshoots is on the path of both.  What is waited for comes within microseconds.  A try that fails has
+// waited for about 2700 clocks: 2^22 of them are some 6 s.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 26); ++i)
+  for (uint32_t i = 0; i < (1u << 22); ++i)
     if (tc::mbar_try_wait(bar, parity)) return true;
   return false;
 }
@@ -353,71 +352,181 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
 }
 
 // ------------------------------------------------------------------------------------------ softmax
-// Columns [c0, c0 + 32) of a query row whose tensor-core sums are not finite in the columns of `bad`, though its scores are: an
-// infinity or NaN among the values, of a key that the row sees or of one that it does not (0 x inf), or sums beyond fp32.  First
-// the values that the row sees are looked through: those columns that hold a NaN or infinity get theirs; what is left is summed
-// again over the keys that the row sees, with the maximum and the sum that the tiles gave and the weights normalised ahead.
-__device__ __noinline__ void redo_columns(const PromptArgs& a, int b, int hq, int hkv, int t, int p, int c0, unsigned bad, float m, float inv) {
-  bf16* dst = a.out + (((size_t)b * a.T + t) * a.Hq + hq) * a.D + c0;
-  const int lo = max(0, p - a.window + 1), ns = min(a.sinks, lo), n = ns + p + 1 - lo;
-  unsigned nan = 0, pos = 0, neg = 0;
-  for (int i = 0; i < n && (bad & ~(nan | (pos & neg))); ++i) {
-    const bf16* vr = a.v.row(b, hkv, i < ns ? i : lo + i - ns) + c0;
+// Rows to be formed again.  The tiles leave a mark in the first column that is concerned, a NaN that no conversion makes: the row's
+// scores are numbers, but not all of the tensor core's sums are.  An infinity or NaN among the values did that, of a key that the row sees or of one
+// that it does not (0 x inf), or sums beyond fp32.
+constexpr unsigned kAgain = 0x7fc5;
+
+// Columns [c0, c0 + 32) of the 32 query rows of a warp (one per lane), in each row those of `bad`.  First the values that the rows
+// see are looked through, a key per lane: columns that hold a NaN or infinity get theirs.  What is left is summed again over
+// the keys that the row sees, a row per lane, with normalised weights; their maximum and sum are formed once per row (`have`).
+struct Again {
+  const PromptArgs& a;
+  int b, hq, hkv, t, p, lo, ns, n;  // the keys that any of the rows sees: the first ns, then those from lo on
+  float m, inv;
+  bool have;
+  static constexpr unsigned kAll = 0xffffffffu;
+  static constexpr int kKeys = 8;   // at a time: as many loads in flight
+  __device__ __forceinline__ int key(int i) const { return i < ns ? i : lo + i - ns; }
+  __device__ __forceinline__ bool sees(int i) const {
+    const int j = key(i);
+    return i < n && j <= p && (j > p - a.window || j < a.sinks);
+  }
+  // scores of keys i0 .. i0 + 7, in units of log2
+  __device__ __forceinline__ void scores(int i0, float (&x)[kKeys]) const {
+    const bf16* qr = a.q.row(b, hq, t);
+    float2 s[kKeys];
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      const uint4 y = *reinterpret_cast<const uint4*>(vr + e);
-      const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+    for (int e = 0; e < kKeys; ++e) s[e] = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int d = 0; d < a.D; d += 8) {
+      const uint4 y = *reinterpret_cast<const uint4*>(qr + d);
 #pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        const unsigned u = (ys[z >> 1] >> (16 * (z & 1))) & 0xffffu;
-        if ((u & 0x7f80u) != 0x7f80u) continue;
-        const unsigned bit = 1u << (e + z);
-        if (u & 0x7fu) nan |= bit;
-        else if (u & 0x8000u) neg |= bit;
-        else pos |= bit;
+      for (int e = 0; e < kKeys; ++e) {
+        const uint4 z = *reinterpret_cast<const uint4*>(a.k.row(b, hkv, key(min(i0 + e, n - 1))) + d);
+        s[e] = __ffma2_rn(unpack_bf16(y.x), unpack_bf16(z.x), s[e]);
+        s[e] = __ffma2_rn(unpack_bf16(y.y), unpack_bf16(z.y), s[e]);
+        s[e] = __ffma2_rn(unpack_bf16(y.z), unpack_bf16(z.z), s[e]);
+        s[e] = __ffma2_rn(unpack_bf16(y.w), unpack_bf16(z.w), s[e]);
       }
     }
-  }
-  nan |= pos & neg;
-  const unsigned sum_again = bad & ~(nan | pos | neg);
-  float acc[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-  if (sum_again) {
-    const bf16* qr = a.q.row(b, hq, t);
-    const float neg_m = m == -INFINITY ? 0.f : -m;
-    for (int i = 0; i < n; ++i) {
-      const int j = i < ns ? i : lo + i - ns;
-      const bf16* kr = a.k.row(b, hkv, j);
-      float s = 0.f;
-      for (int d = 0; d < a.D; d += 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(qr + d), y = *reinterpret_cast<const uint4*>(kr + d);
-        const unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    for (int e = 0; e < kKeys; ++e) x[e] = __fmul_rn(s[e].x + s[e].y, a.scale_log2);
+  }
+  __device__ __forceinline__ void columns(int c0, unsigned bad, int lane) {
+    unsigned nan = 0, pos = 0, neg = 0;
+#pragma unroll 2
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      unsigned is_nan = 0, is_pos = 0, is_neg = 0;  // of the lane's key
+      if (i0 + lane < n) {
+        const uint4* vr = reinterpret_cast<const uint4*>(a.v.row(b, hkv, key(i0 + lane)) + c0);
+        uint4 y[4];
+        unsigned top = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16(xs[e]), h = unpack_bf16(ys[e]);
-          s = fmaf(f.x, h.x, fmaf(f.y, h.y, s));
+          y[e] = vr[e];
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(y[e].x & 0x7fff7fffu, y[e].y & 0x7fff7fffu), __vmaxu2(y[e].z & 0x7fff7fffu, y[e].w & 0x7fff7fffu)));
+        }
+        if (max(top & 0xffffu, top >> 16) >= 0x7f80u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned ys[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+              const unsigned u = (ys[z >> 1] >> (16 * (z & 1))) & 0xffffu, bit = 1u << (8 * e + z);
+              if ((u & 0x7fffu) > 0x7f80u) is_nan |= bit;
+              else if (u == 0x7f80u) is_pos |= bit;
+              else if (u == 0xff80u) is_neg |= bit;
+            }
+          }
         }
       }
-      const float w = ex2(fmaf(s, a.scale_log2, neg_m)) * inv;
-      const bf16* vr = a.v.row(b, hkv, j) + c0;
+      unsigned hits = __ballot_sync(kAll, (is_nan | is_pos | is_neg) != 0);
+      if (hits == 0) continue;
+      for (; hits; hits &= hits - 1) {
+        const int src = __ffs(hits) - 1;
+        const unsigned x = __shfl_sync(kAll, is_nan, src), y = __shfl_sync(kAll, is_pos, src), z = __shfl_sync(kAll, is_neg, src);
+        if (sees(i0 + src)) { nan |= x; pos |= y; neg |= z; }
+      }
+      if (!__any_sync(kAll, bad & ~(nan | (pos & neg)))) break;  // (settled whatever follows)
+    }
+    nan |= pos & neg;
+    float acc[32];
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        const uint4 y = *reinterpret_cast<const uint4*>(vr + e);
-        const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    if (__any_sync(kAll, bad & ~(nan | pos | neg))) {
+      if (!have) {
+        float sum = 0.f;
+        m = -INFINITY;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += kKeys) {
+          float x[kKeys], top = m;
+          scores(i0, x);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const float2 h = unpack_bf16(ys[z]);
-          acc[e + 2 * z] = fmaf(w, h.x, acc[e + 2 * z]);
-          acc[e + 2 * z + 1] = fmaf(w, h.y, acc[e + 2 * z + 1]);
+          for (int e = 0; e < kKeys; ++e) {
+            if (!sees(i0 + e)) x[e] = -INFINITY;
+            top = fmaxf(top, x[e]);
+          }
+          if (top == -INFINITY) continue;
+          sum *= ex2(m - top);
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e) sum += ex2(x[e] - top);
+          m = top;
+        }
+        inv = 1.0f / sum;
+        have = true;
+      }
+#pragma unroll 1
+      for (int i0 = 0; i0 < n; i0 += kKeys) {
+        float x[kKeys];
+        scores(i0, x);
+#pragma unroll
+        for (int e = 0; e < kKeys; ++e) {
+          const float w = ex2(x[e] - m) * inv;
+          const uint4* vr = reinterpret_cast<const uint4*>(a.v.row(b, hkv, key(min(i0 + e, n - 1))) + c0);
+          const bool seen = sees(i0 + e);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const uint4 y = vr[z];
+            const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float2 h = unpack_bf16(ys[u]);
+              if (seen) {
+                acc[8 * z + 2 * u] = fmaf(w, h.x, acc[8 * z + 2 * u]);
+                acc[8 * z + 2 * u + 1] = fmaf(w, h.y, acc[8 * z + 2 * u + 1]);
+              }
+            }
+          }
+          asm volatile("" ::: "memory");  // (one key's values at a time: registers)
         }
       }
     }
-  }
+    bf16* dst = a.out + (((size_t)b * a.T + t) * a.Hq + hq) * a.D + c0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (bad >> i & 1)
-      dst[i] = __float2bfloat16_rn((nan >> i & 1) ? __int_as_float(0x7fffffff) : (pos >> i & 1) ? INFINITY : (neg >> i & 1) ? -INFINITY : acc[i]);
+    for (int i = 0; i < 32; ++i)
+      if (bad >> i & 1)
+        dst[i] = __float2bfloat16_rn((nan >> i & 1) ? __int_as_float(0x7fffffff) : (pos >> i & 1) ? INFINITY : (neg >> i & 1) ? -INFINITY : acc[i]);
+  }
+};
+
+// The marked rows of a softmax warp, once its tiles are done: nobody waits for it any more, however long it takes.  For 32 rows of
+// 128 channels: 12 ns per key and 32 columns to look through the values, 2.1 us per key to sum 32 columns again, 1.1 us for each
+// further 32 (of 8192 keys 17.7 ms, all columns 45 ms).  Inside the tiles' loop a call took 2 to 4 % of every prompt's time.
+template <bool LISTED>
+__device__ __noinline__ void revisit(const PromptArgs& a, const int* pre, int n_items, int I, int row, int lane) {
+  constexpr unsigned kAll = 0xffffffffu;
+#pragma unroll 1
+  for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
+    const Item<LISTED> it(a, pre, x);
+    const int t = it.pick(it.t0, I) + row, p = a.S - a.T + t, hq = it.pick(it.hq, I);
+    bool again = false;
+    unsigned bad[4] = {0, 0, 0, 0};  // columns that hold no number
+    if (t < a.T && p < it.len) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.out + (((size_t)it.b * a.T + t) * a.Hq + hq) * a.D);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (e * 8 >= a.D) break;
+        const uint4 y = src[e];
+        const unsigned ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          const unsigned u = (ys[z >> 1] >> (16 * (z & 1))) & 0xffffu;
+          if ((u & 0x7f80u) == 0x7f80u) bad[e >> 2] |= 1u << (8 * (e & 3) + z);
+          again |= u == kAgain;
+        }
+      }
+    }
+    if (!__any_sync(kAll, again)) continue;
+    const int p_lo = __reduce_min_sync(kAll, again ? p : 0x7fffffff), p_hi = __reduce_max_sync(kAll, again ? p : -1);
+    const int lo = max(0, p_lo - a.window + 1), ns = min(a.sinks, lo);
+    Again rows{a, it.b, hq, it.hkv, again ? t : 0, again ? p : -1, lo, ns, ns + p_hi + 1 - lo, 0.f, 0.f, false};
+#pragma unroll 1
+    for (int c0 = 0; c0 < a.D; c0 += 32) {
+      const unsigned mine = !again ? 0 : c0 < 64 ? (c0 < 32 ? bad[0] : bad[1]) : (c0 < 96 ? bad[2] : bad[3]);
+      if (__any_sync(kAll, mine)) rows.columns(c0, mine, lane);
+    }
+  }
 }
 
 template <int DP, bool LISTED>
@@ -427,6 +536,7 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
   const uint32_t col_s = lane_addr + I * 128, col_o = lane_addr + PC<DP>::kColO + I * DP;
   const float sc = a.scale_log2;
   int slot = 0, round = 0, n = 0, ni = 0;
+  bool marked = false;
   for (int x = blockIdx.x; x < n_items; x += gridDim.x) {
     const Item<LISTED> it(a, pre, x);
     const int t = it.pick(it.t0, I) + row, p0 = a.S - a.T + it.pick(it.t0, I), p = p0 + row;
@@ -550,18 +660,18 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
     const bool valid = mine && p < it.len;
     if (poison || m_run == -INFINITY) l_run = __int_as_float(0x7fffffff);  // (no score above -inf: 0 / 0)
     const float inv = valid ? 1.0f / l_run : 0.f;
-    unsigned bad[DP / 32];
+    float largest = 0.f;  // magnitude among the sums, NaN if there is one
 #pragma unroll
     for (int hb = 0; hb < DP / 32; ++hb) {
       uint32_t o[32];
       tc::tmem_ld32(col_o + hb * 32, o);
       tc::tmem_ld_wait();
-      bad[hb] = 0;
       if (hb * 32 < a.D && mine) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!(fabsf(__uint_as_float(o[i])) < INFINITY)) bad[hb] |= 1u << i;
+        for (int i = 0; i < 32; i += 2) {
+          largest = max3(largest, fabsf(__uint_as_float(o[i])), fabsf(__uint_as_float(o[i + 1])));
           o[i] = valid ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+          o[i + 1] = valid ? __float_as_uint(__uint_as_float(o[i + 1]) * inv) : 0u;
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
@@ -577,13 +687,15 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
     tc::tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&bars->o_free[I]);
-    if (valid && l_run < INFINITY) {
-#pragma unroll
-      for (int hb = 0; hb < DP / 32; ++hb)
-        if (bad[hb]) redo_columns(a, it.b, it.pick(it.hq, I), it.hkv, t, p, hb * 32, bad[hb], m_run, inv);
+    if (valid && l_run < INFINITY && !(largest < INFINITY)) {
+      unsigned short* at = reinterpret_cast<unsigned short*>(dst);
+      int c = 0;
+      while (c + 1 < a.D && (at[c] & 0x7f80u) != 0x7f80u) ++c;  // (what is not finite is stored so)
+      at[c] = kAgain;
+      marked = true;
     }
-    __syncwarp();
   }
+  if (__any_sync(0xffffffffu, marked)) revisit<LISTED>(a, pre, n_items, I, row, lane);
   return true;
 }
 

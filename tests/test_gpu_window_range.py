@@ -171,3 +171,75 @@ def test_prompt_values_far_below_the_maximum_weigh_nothing(dim, far):
     assert float(want.abs().max()) < 10
     tol = (2 * wh.U_BF16 + 2.0 ** -8) * mag + 2.0 ** -20  # scores up to 2^10: as in the test of scores far apart
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+def _timed(fn):
+    fn()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = fn()
+    end.record()
+    torch.cuda.synchronize()
+    return out, start.elapsed_time(end)
+
+
+def test_prompt_an_infinity_that_every_row_sees_costs_little():
+    """An infinity in a sink: every row's values are looked through, in steps of 32 keys of about one round trip to memory
+    (1000 clocks): 1024 steps of half a microsecond per row of 32768 keys, two rounds of work items."""
+    from kvm_paper_b200 import window
+    g = _gen(56)
+    T, D = 32768, 64
+    q, k, v = wh.heads_data(g, 1, 2, T, D), wh.heads_data(g, 1, 1, T, D), wh.heads_data(g, 1, 1, T, D)
+    v[0, 0, 1, 9] = math.inf
+    got, ms = _timed(lambda: window.window_attention(q, k, v, window=20000, sinks=4))
+    assert ms < 10.0
+    got = got.view(T, 2, D)
+    assert bool(torch.isinf(got[1:, :, 9]).all()) and bool((got[1:, :, 9] > 0).all())
+    got[1:, :, 9] = 0
+    assert bool(torch.isfinite(got).all())
+    v[0, 0, 1, 9] = 0
+    plain = window.window_attention(q, k, v, window=20000, sinks=4).view(T, 2, D)
+    plain[1:, :, 9] = 0
+    assert torch.equal(got, plain)
+    window.check_status()
+
+
+def test_prompt_a_value_that_part_of_a_tile_does_not_see_costs_little():
+    """Infinities that most of their tile's rows do not see: those rows are formed again from what they see, twice 8064 keys
+    (maximum and sum, then values) of at most 2000 clocks, 18 ms; half as much again is allowed."""
+    from kvm_paper_b200 import window
+    g = _gen(57)
+    T, D = 8192, 128
+    q, k, v = wh.heads_data(g, 1, 4, T, D), wh.heads_data(g, 1, 2, T, D), wh.heads_data(g, 1, 2, T, D)
+    v[0, 0, 8180, 100] = math.inf
+    v[0, 1, 8150, 3] = math.nan
+    got, ms = _timed(lambda: window.window_attention(q, k, v, window=None))
+    assert ms < 27.0
+    got = got.view(1, T, 4, D)
+    assert bool(torch.isnan(got[0, 8150:, 2:, 3]).all()) and bool(torch.isinf(got[0, 8180:, :2, 100]).all())
+    rows = slice(8100, T)
+    want, mag = wh.prompt(q[:, :, rows], k, v, None, 0)
+    got = got[:, rows]
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    wh.assert_near(torch.where(fine, got.double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
+    window.check_status()
+
+
+@pytest.mark.parametrize("dim,hq,hkv", [(128, 3, 1), (64, 2, 2), (32, 4, 1)])
+@pytest.mark.parametrize("window_,sinks", [(None, 0), (40, 70), (200, 3), (7, 0)])
+def test_prompt_scattered_infinities_and_values_near_the_largest_number(dim, hq, hkv, window_, sinks):
+    """Both signs in a column, in sinks, in the window and behind it; columns whose sums pass fp32's range beside them."""
+    from kvm_paper_b200 import window
+    g = _gen(58 + dim)
+    T = 450
+    q, k, v = wh.heads_data(g, 1, hq, T, dim), wh.heads_data(g, 1, hkv, T, dim), wh.heads_data(g, 1, hkv, T, dim)
+    v[..., 8:12] *= 5e37
+    for i, j in enumerate((0, 2, 31, 32, 69, 70, 127, 128, 200, 255, 256, 300, 301, 440, 449)):
+        v[0, i % hkv, j, (5 * i) % dim] = (math.inf, -math.inf, math.nan)[i % 3]
+        v[0, i % hkv, j, 20] = math.inf if i % 2 else -math.inf
+    got = window.window_attention(q, k, v, window=window_, sinks=sinks).view(1, T, hq, dim)
+    want, mag = wh.prompt(q, k, v, window_, sinks)
+    wh.assert_near(torch.where(torch.isinf(got), 0.0, got.double()), torch.where(torch.isinf(want), 0.0, want), torch.where(torch.isinf(want), 0.0, mag))
+    assert torch.equal(torch.where(torch.isinf(got), got.double(), 0.0), torch.where(torch.isinf(want), want, 0.0))
+    window.check_status()
