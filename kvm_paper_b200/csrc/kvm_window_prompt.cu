@@ -355,7 +355,12 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
 // Rows to be formed again.  The tiles leave a mark in the first column that is concerned, a NaN that no conversion makes: the row's
 // scores are numbers, but not all of the tensor core's sums are.  An infinity or NaN among the values did that, of a key that the row sees or of one
 // that it does not (0 x inf), or sums beyond fp32.
-constexpr unsigned kAgain = 0x7fc5;
+// Another mark in the first column asks for all of the row's columns: its maximum is beyond 2^16.  The tiles form a weight from a fused
+// product and difference, which lies off the rounded maximum by up to half a step: 2^-8 there, from 2^31 on more than a
+// weight holds.  The second pass rounds every score as it rounds the maximum.  (As a variant of the tiles' weights it took 1 to 5 % of
+// every prompt's time.)
+constexpr unsigned kAgain = 0x7fc5, kAllAgain = 0x7fc6;
+constexpr float kFar = 0x1p16f;
 
 // Columns [c0, c0 + 32) of the 32 query rows of a warp (one per lane), in each row those of `bad`.  First the values that the rows
 // see are looked through, a key per lane: columns that hold a NaN or infinity get theirs.  What is left is summed again over
@@ -513,7 +518,8 @@ __device__ __noinline__ void revisit(const PromptArgs& a, const int* pre, int n_
         for (int z = 0; z < 8; ++z) {
           const unsigned u = (ys[z >> 1] >> (16 * (z & 1))) & 0xffffu;
           if ((u & 0x7f80u) == 0x7f80u) bad[e >> 2] |= 1u << (8 * (e & 3) + z);
-          again |= u == kAgain;
+          again |= u == kAgain || u == kAllAgain;
+          if (u == kAllAgain) bad[0] = bad[1] = bad[2] = bad[3] = 0xffffffffu;
         }
       }
     }
@@ -687,7 +693,10 @@ __device__ __forceinline__ bool softmax(const PromptArgs& a, const int* pre, int
     tc::tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&bars->o_free[I]);
-    if (valid && l_run < INFINITY && !(largest < INFINITY)) {
+    if (valid && !poison && fabsf(m_run) > kFar && m_run > -INFINITY) {
+      *reinterpret_cast<unsigned short*>(dst) = kAllAgain;
+      marked = true;
+    } else if (valid && l_run < INFINITY && !(largest < INFINITY)) {
       unsigned short* at = reinterpret_cast<unsigned short*>(dst);
       int c = 0;
       while (c + 1 < a.D && (at[c] & 0x7f80u) != 0x7f80u) ++c;  // (what is not finite is stored so)

@@ -93,9 +93,9 @@ def _one_hot(up, sign, heads, rows, dim):
 
 @pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("up", [10, 13, 14, 15, 16, 17, 18, 19, 20, 30, 50, 60])
+@pytest.mark.parametrize("up", [4, 6, 8, 9, 10, 13, 14, 15, 16, 17, 18, 19, 20, 30, 50, 60])
 def test_token_scores_of_any_size(bits, sign, up):
-    """Scores of 2^21 to 2^121, all of them finite: the keys with the largest one share the whole weight."""
+    """Scores of 2^9 to 2^121, all of them finite: the keys with the largest one share the weight."""
     from kvm_paper_b200 import window
     g = _gen(60 + up)
     for dim, group, n in ((64, 3, 500), (128, 9, 900), (32, 8, 9000)):
@@ -243,3 +243,18 @@ def test_prompt_scattered_infinities_and_values_near_the_largest_number(dim, hq,
     wh.assert_near(torch.where(torch.isinf(got), 0.0, got.double()), torch.where(torch.isinf(want), 0.0, want), torch.where(torch.isinf(want), 0.0, mag))
     assert torch.equal(torch.where(torch.isinf(got), got.double(), 0.0), torch.where(torch.isinf(want), want, 0.0))
     window.check_status()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("up", [4, 6, 8, 9, 10, 13, 14, 15, 16, 17, 18, 19, 20, 30, 50, 60])
+def test_prompt_scores_of_any_size(sign, up):
+    from kvm_paper_b200 import window
+    g = _gen(80 + up)
+    for dim, hq, T, window_, sinks in ((64, 2, 500, None, 0), (128, 1, 420, 300, 128), (32, 4, 300, 100, 3)):
+        k, v = _one_hot(up, sign, 1, T, dim), wh.heads_data(g, 1, 1, T, dim)
+        q = torch.zeros(1, hq, T, dim, device="cuda", dtype=torch.bfloat16)
+        q[..., 5] = (1 + torch.arange(T, device="cuda") % 8 / 8) * 2.0 ** up
+        for scale in (None, 1.0):
+            got = window.window_attention(q, k, v, window=window_, sinks=sinks, scale=scale)
+            want, mag = wh.prompt(q, k, v, window_, sinks, scale)
+            wh.assert_near(got.view(1, T, hq, dim), want, mag)
