@@ -453,7 +453,8 @@ size_t kvm_window_cache_bytes(const kvm_window_cache* cache);
 /* Writes tokens [position, position + length) of every sequence: k, v [batch, n_kv_heads, n_tokens, head_dim], of which the
  * first `length` are taken.  positions_dev / lengths_dev: int32 [batch] on the device, or NULL: `position` / `length` for all
  * sequences.  A negative position, or a length of 0, leaves the sequence as it is.  Tokens that later tokens of the same
- * call push out are not written.  Positions stay below 2^31 - n_tokens (one that does not leaves its sequence as it is). */
+ * call push out are not written.  k and v are not rows of the cache itself that the call writes.  Positions stay below
+ * 2^31 - n_tokens (one that does not leaves its sequence as it is). */
 typedef struct kvm_window_write_args {
   const kvm_window_cache* cache;
   kvm_tensor4 k, v;
@@ -472,7 +473,8 @@ int kvm_window_cache_read(const kvm_window_cache* cache, const int32_t* lengths_
  * kv head.  Without a new token (k_new.ptr and v_new.ptr NULL) lengths are the tokens of the sequences, the query's own among
  * them; with one they are its positions, and it is written to the cache on the way.  A sequence of no tokens (length 0, or
  * position -1) gets zeros.  The workspace (none where kvm_window_attend_workspace_bytes() says 0) holds partial results of one
- * call; calls in flight at the same time need one each.  0 < scale < 1e38 multiplies the scores. */
+ * call; calls in flight at the same time need one each.  0 < scale < 1e38 multiplies the scores.  out shares no memory with the
+ * inputs, but may lie exactly in the place of q. */
 typedef struct kvm_window_attend_args {
   const kvm_window_cache* cache;
   kvm_tensor4 q, k_new, v_new;
@@ -490,7 +492,7 @@ int kvm_window_attend(const kvm_window_attend_args* args, void* stream);
  * head_dim], out bf16 [batch, n_queries, n_q_heads * head_dim]; fewer than 2^30 keys.  Query t stands at position n_keys -
  * n_queries + t.
  * lengths_dev (int32 [batch], or NULL: n_keys): tokens of each sequence; tokens behind them are padding, never looked at, and
- * their output rows are zeros. */
+ * their output rows are zeros.  out shares no memory with the inputs. */
 typedef struct kvm_window_prompt_args {
   kvm_tensor4 q, k, v;
   const int32_t* lengths_dev;

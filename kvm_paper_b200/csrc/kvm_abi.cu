@@ -267,6 +267,15 @@ int check_scale(float scale) {
   return KVM_OK;
 }
 
+// Do the `bytes` of an output lie anywhere between an input's first and last element?  (An output is one contiguous piece.)
+bool overlaps(const void* out, int64_t bytes, const kvm_tensor4& t, int batch, int heads, int64_t rows, int head_dim) {
+  int64_t lo = 0, hi = head_dim;
+  const int64_t last[3] = {(batch - 1) * t.stride_b, (heads - 1) * t.stride_h, (rows - 1) * t.stride_t};
+  for (int64_t x : last) (x < 0 ? lo : hi) += x;
+  const intptr_t at = (intptr_t)out, base = (intptr_t)t.ptr;
+  return at < base + hi * 2 && base + lo * 2 < at + bytes;
+}
+
 int check_groups(const kvm_window_cache* c, int n_q_heads) {
   if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads)
     return fail(KVM_ERR_BAD_ARGUMENT, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, c->n_kv_heads);
@@ -587,6 +596,15 @@ int kvm_window_attend(const kvm_window_attend_args* a, void* stream) {
   const size_t need = window_token_workspace(cache->head_dim, cache->bits, w, G);
   if (need && (!a->workspace || ((uintptr_t)a->workspace) % 16 || a->workspace_bytes < need))
     return fail(KVM_ERR_CAPACITY, "kvm_window_attend: workspace of %zu bytes (needs %zu, 16-byte aligned)", a->workspace_bytes, need);
+  // (in place of the queries it may be: a kv row's are read before its output is written)
+  const int D = cache->head_dim;
+  const int64_t bytes = (int64_t)cache->batch * a->n_q_heads * D * 2;
+  const bool in_place = a->out == a->q.ptr && (a->n_q_heads == 1 || a->q.stride_h == D) &&
+                        (cache->batch == 1 || a->q.stride_b == (int64_t)a->n_q_heads * D);
+  if ((!in_place && overlaps(a->out, bytes, a->q, cache->batch, a->n_q_heads, 1, D)) ||
+      (a->k_new.ptr && (overlaps(a->out, bytes, a->k_new, cache->batch, cache->n_kv_heads, 1, D) ||
+                        overlaps(a->out, bytes, a->v_new, cache->batch, cache->n_kv_heads, 1, D))))
+    return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attend: out must not share memory with q (but lie exactly in its place), k or v");
   int* status = nullptr;
   if (int rc = window_status_word(&status)) return rc;
   const cudaError_t e = window_token_dispatch(cache->head_dim, cache->bits, w, G, to_dev(a->q), to_dev(a->k_new), to_dev(a->v_new),
@@ -620,6 +638,11 @@ int kvm_window_attention(const kvm_window_prompt_args* a, void* stream) {
         ((i ? a->n_keys : a->n_queries) > 1 && in[i]->stride_t <= 0))
       return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: strides must be positive");
   if (!a->out || ((uintptr_t)a->out) % 16) return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must be 16-byte aligned and not NULL");
+  const int64_t bytes = a->batch * a->n_queries * a->n_q_heads * a->head_dim * 2;
+  if (overlaps(a->out, bytes, a->q, a->batch, a->n_q_heads, a->n_queries, a->head_dim) ||
+      overlaps(a->out, bytes, a->k, a->batch, a->n_kv_heads, a->n_keys, a->head_dim) ||
+      overlaps(a->out, bytes, a->v, a->batch, a->n_kv_heads, a->n_keys, a->head_dim))
+    return fail(KVM_ERR_BAD_ARGUMENT, "kvm_window_attention: out must not share memory with q, k or v");
   int* status = nullptr;
   if (int rc = window_status_word(&status)) return rc;
   const int w = (int)(a->window < a->n_keys ? a->window : a->n_keys), s = (int)(a->sinks < a->n_keys ? a->sinks : a->n_keys);

@@ -119,7 +119,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     what ``WindowCache.read`` returns: positions only count relative to each other, as long as the sinks and the last
     ``window - 1`` tokens are there.)  ``window`` None: every earlier token is visible.  ``lengths`` (int32 [B]): tokens of each
     sequence, S at most; what lies behind them is padding, is never looked at, and its output rows are zeros.
-    Returns [B,T,Hq*D] (``out`` if given)."""
+    Returns [B,T,Hq*D] (``out`` if given, which must not share memory with q, k or v)."""
     B, Hq, T, D = _shape4(q, "q", "[B,Hq,T,D]")
     _, Hkv, S, _ = _shape4(k, "k", "[B,Hkv,S,D]")
     dev = q.device
@@ -223,7 +223,7 @@ class WindowCache:
 
     def attend(self, q: torch.Tensor, lengths, *, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """One query per sequence over the cached tokens: q [B,Hq,1,D], ``lengths`` the tokens of the sequences, the query's own
-        among them.  Returns [B,1,Hq*D]; a sequence of no tokens gets zeros."""
+        among them.  Returns [B,1,Hq*D] (``out`` if given; it may be q's own memory); a sequence of no tokens gets zeros."""
         none = (0, 0, 0, 0)
         return self._attend(q, none, none, _counts(lengths, "lengths", self.batch, self.device, 0, 2**31 - 1), scale, out)
 

@@ -258,3 +258,25 @@ def test_prompt_scores_of_any_size(sign, up):
             got = window.window_attention(q, k, v, window=window_, sinks=sinks, scale=scale)
             want, mag = wh.prompt(q, k, v, window_, sinks, scale)
             wh.assert_near(got.view(1, T, hq, dim), want, mag)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_tokens_in_place_of_their_queries(bits):
+    """Rows in one share and rows that are cut; the prompt call refuses it."""
+    from kvm_paper_b200 import window
+    g = _gen(90)
+    for B, n in ((5, 40), (1, 30000)):
+        c = window.WindowCache(B, 2, 64, window=n, bits=bits)
+        c.write(wh.heads_data(g, B, 2, n, 64), wh.heads_data(g, B, 2, n, 64), 0)
+        k1, v1 = wh.heads_data(g, B, 2, 1, 64), wh.heads_data(g, B, 2, 1, 64)
+        store = torch.randn(B, 1, 8 * 64, device="cuda", generator=g).bfloat16()
+        q = store.view(B, 1, 8, 64).transpose(1, 2)
+        want = c.step(q.clone(), k1, v1, n)
+        assert c.attend(q.clone(), n + 1).equal(want)
+        assert c.step(q, k1, v1, n, out=store) is store and store.equal(want)
+        with pytest.raises(ValueError, match="share memory"):
+            c.attend(q[:, 0:2], 3, out=store.view(-1)[64:64 + B * 128].view(B, 1, 128))
+    q, k = wh.heads_data(g, 2, 4, 50, 64), wh.heads_data(g, 2, 4, 50, 64)
+    for t in (q, k):
+        with pytest.raises(ValueError, match="share memory"):
+            window.window_attention(q, k, k, window=9, out=t.transpose(1, 2).reshape(2, 50, 256))

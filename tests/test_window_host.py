@@ -117,3 +117,19 @@ def test_scales_beyond_the_range_are_refused():
 def test_packed_blocks_are_what_the_structures_hold(cls):
     values = [0.25 if t is C.c_float else 2**31 - 1 - i if t is C.c_int32 else 2**40 + i for i, (_, t) in enumerate(cls._fields_)]
     assert _lib.packer(cls)(*values) == bytes(cls(*values))
+
+
+def test_outputs_over_inputs_are_refused():
+    """The prompt call reads its inputs again behind its first outputs; the token call may write in place of the queries."""
+    lib, c = _lib.load(), _cache(batch=2, n_kv_heads=1, window=1 << 10)
+    at = 1 << 20
+    q, k, v = (at, 8 * 128, 64, 128), (at + (1 << 16), 8 * 64, 512, 64), (at + (1 << 17), 8 * 64, 512, 64)  # [2,2,8,64], [2,1,8,64]
+    size = 2 * 8 * 2 * 64 * 2
+    for out in (at, at + size - 16, at - size + 16, k[0], k[0] + 2 * 8 * 64 * 2 - 16, v[0] - size + 16):
+        a = _lib.KvmWindowPromptArgs(*q, *k, *v, None, out, 8, 8, 4, 0, 2, 2, 1, 64, 0.125)
+        assert lib.kvm_window_attention(C.addressof(a), None) == 1 and "share memory" in _err(), out
+    one = 2 * 2 * 64 * 2
+    q1, k1, v1 = (at, 128, 64, 64), (at + 4096, 64, 64, 64), (at + 8192, -64, 64, 64)
+    for q2, out in ((q1, at + 16), (q1, at - 16), (q1, k1[0]), (q1, v1[0] + 128 - 16), (q1, v1[0] - one - 128 + 16), ((at, 256, 64, 64), at), ((at, 128, 128, 64), at)):
+        a = _lib.KvmWindowAttendArgs(C.addressof(c), *q2, *k1, *v1, None, out, 1 << 24, 1 << 30, 2, 4, 0.125)
+        assert lib.kvm_window_attend(C.addressof(a), None) == 1 and "share memory" in _err(), (q2, out)
