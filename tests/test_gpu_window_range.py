@@ -280,3 +280,22 @@ def test_tokens_in_place_of_their_queries(bits):
     for t in (q, k):
         with pytest.raises(ValueError, match="share memory"):
             window.window_attention(q, k, k, window=9, out=t.transpose(1, 2).reshape(2, 50, 256))
+
+
+@pytest.mark.parametrize("order", [(1, 0, 2), (2, 0, 1), (2, 1, 0), (1, 2, 0), (0, 2, 1)])
+def test_strides_in_any_order(order):
+    """Storage of batch, heads and tokens in any order (channels last), read where it lies."""
+    from kvm_paper_b200 import window
+    g = _gen(59)
+    back = [order.index(i) for i in range(3)] + [3]
+    for B, H, T, D in ((3, 4, 150, 64), (2, 2, 40, 32), (2, 3, 129, 128)):
+        q, k, v = (torch.randn(*[(B, H, T)[i] for i in order], D, device="cuda", generator=g).bfloat16().permute(back) for _ in range(3))
+        plain = [t.contiguous() for t in (q, k, v)]
+        lens = _ints([T, T // 2, 1][:B])
+        for kw in (dict(window=33, sinks=2), dict(window=None, lengths=lens)):
+            assert torch.equal(window.window_attention(q, k, v, **kw), window.window_attention(*plain, **kw))
+        for bits in (4, 16):
+            c, c2 = (window.WindowCache(B, H, D, window=50, sinks=2, bits=bits) for _ in range(2))
+            c.write(k, v, 0, lengths=lens), c2.write(*plain[1:], 0, lengths=lens)
+            assert torch.equal(c.step(q[:, :, :1], k[:, :, :1], v[:, :, :1], lens), c2.step(*(t[:, :, :1].contiguous() for t in plain), lens))
+            assert all(torch.equal(x, y) for x, y in zip(c.read(lens + 1), c2.read(lens + 1)))
