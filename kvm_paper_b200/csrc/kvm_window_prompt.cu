@@ -363,8 +363,9 @@ constexpr unsigned kAgain = 0x7fc5, kAllAgain = 0x7fc6;
 constexpr float kFar = 0x1p16f;
 
 // Columns [c0, c0 + 32) of the 32 query rows of a warp (one per lane), in each row those of `bad`.  First the values that the rows
-// see are looked through, a key per lane: columns that hold a NaN or infinity get theirs.  What is left is summed again over
-// the keys that the row sees, a row per lane, with normalised weights; their maximum and sum are formed once per row (`have`).
+// see are looked through, a key per lane: columns that hold a NaN or infinity get theirs (NaN for an infinity whose weight is 0).
+// What is left is summed again over the keys that the row sees, a row per lane, with normalised weights; their maximum and sum
+// are formed once per row (`have`).
 struct Again {
   const PromptArgs& a;
   int b, hq, hkv, t, p, lo, ns, n;  // the keys that any of the rows sees: the first ns, then those from lo on
@@ -397,6 +398,20 @@ struct Again {
     }
 #pragma unroll
     for (int e = 0; e < kKeys; ++e) x[e] = __fmul_rn(s[e].x + s[e].y, a.scale_log2);
+  }
+  // is the score of key j -inf?
+  __device__ __forceinline__ bool weightless(int j) const {
+    const bf16 *qr = a.q.row(b, hq, t), *kr = a.k.row(b, hkv, j);
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int d = 0; d < a.D; d += 8) {
+      const uint4 y = *reinterpret_cast<const uint4*>(qr + d), z = *reinterpret_cast<const uint4*>(kr + d);
+      s = __ffma2_rn(unpack_bf16(y.x), unpack_bf16(z.x), s);
+      s = __ffma2_rn(unpack_bf16(y.y), unpack_bf16(z.y), s);
+      s = __ffma2_rn(unpack_bf16(y.z), unpack_bf16(z.z), s);
+      s = __ffma2_rn(unpack_bf16(y.w), unpack_bf16(z.w), s);
+    }
+    return s.x + s.y == -INFINITY;
   }
   __device__ __forceinline__ void columns(int c0, unsigned bad, int lane) {
     unsigned nan = 0, pos = 0, neg = 0;
@@ -431,7 +446,11 @@ struct Again {
       for (; hits; hits &= hits - 1) {
         const int src = __ffs(hits) - 1;
         const unsigned x = __shfl_sync(kAll, is_nan, src), y = __shfl_sync(kAll, is_pos, src), z = __shfl_sync(kAll, is_neg, src);
-        if (sees(i0 + src)) { nan |= x; pos |= y; neg |= z; }
+        if (!sees(i0 + src)) continue;
+        nan |= x;
+        if ((y | z) == 0) continue;
+        if (weightless(key(i0 + src))) nan |= y | z;  // (0 x inf, of a key that is seen)
+        else { pos |= y; neg |= z; }
       }
       if (!__any_sync(kAll, bad & ~(nan | (pos & neg)))) break;  // (settled whatever follows)
     }

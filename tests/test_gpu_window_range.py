@@ -299,3 +299,23 @@ def test_strides_in_any_order(order):
             c.write(k, v, 0, lengths=lens), c2.write(*plain[1:], 0, lengths=lens)
             assert torch.equal(c.step(q[:, :, :1], k[:, :, :1], v[:, :, :1], lens), c2.step(*(t[:, :, :1].contiguous() for t in plain), lens))
             assert all(torch.equal(x, y) for x, y in zip(c.read(lens + 1), c2.read(lens + 1)))
+
+
+@pytest.mark.parametrize("dim", [128, 64, 32])
+def test_prompt_an_infinity_without_a_weight_is_nan(dim):
+    """A key that is seen with a score of -inf has the weight 0: an infinity among its values gives 0 x inf, where another key's
+    gives an infinity."""
+    from kvm_paper_b200 import window
+    g = _gen(91)
+    T = 300
+    q, k, v = (wh.heads_data(g, 1, 2, T, dim) for _ in range(3))
+    q[..., 0] = 1.0
+    k[0, 0, 150, 0], k[0, 1, 20:25, 0] = -math.inf, -math.inf
+    v[0, 0, 150, 3], v[0, 0, 40, 7], v[0, 1, 22, 9], v[0, 1, 23, 10], v[0, 1, 25, 10] = math.inf, -math.inf, -math.inf, math.inf, math.inf
+    for window_, sinks in ((None, 0), (60, 24)):
+        got = window.window_attention(q, k, v, window=window_, sinks=sinks).view(1, T, 2, dim)
+        want, mag = wh.prompt(q, k, v, window_, sinks)
+        inf = torch.isinf(want)
+        assert int(inf.sum()) > 50 and int(torch.isnan(want).sum()) > 50
+        assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), want[inf])
+        wh.assert_near(torch.where(inf, 0.0, got.double()), torch.where(inf, 0.0, want), torch.where(inf, 0.0, mag))
