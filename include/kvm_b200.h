@@ -504,7 +504,8 @@ typedef struct kvm_window_prompt_args {
 int kvm_window_attention(const kvm_window_prompt_args* args, void* stream);
 
 /* Device-side condition of the window kernels on the current device since the last call (synchronises the stream):
- * KVM_ERR_DEVICE_TIMEOUT if a bounded wait ran out.  One word per device, in the library. */
+ * KVM_ERR_DEVICE_TIMEOUT if a bounded wait ran out, whoever's call it was in.  One word per device, in the library, cleared by
+ * the call that reports it. */
 int kvm_window_status(void* stream);
 
 /* Description of the last error of the calling thread ("" if none). */

@@ -66,8 +66,8 @@ __device__ __forceinline__ unsigned short group_scale(unsigned amax_bits, float&
   return (unsigned short)(u >> 16);
 }
 // x / s to within 2^-14, exact where it lies on the border between two levels: x has 8 and s 6 significant bits, so a
-// quotient off the border is at least 2^-9 away from it, and the product with the reciprocal errs by less than 2^-19.  (A sum
-// in [512, 1024) is a multiple of 2^-14.)
+// quotient off the border is at least 2^-10 away from it (255 / 1024 beside 1 / 4, the nearest of all mantissas and borders), and
+// the product with the reciprocal errs by less than 2^-19.  (A sum in [512, 1024) is a multiple of 2^-14.)
 __device__ __forceinline__ float2 levels_of(unsigned x2, float inv) {
   return __fadd2_rn(__ffma2_rn(unpack_bf16(x2), make_float2(inv, inv), make_float2(768.f, 768.f)), make_float2(-768.f, -768.f));
 }

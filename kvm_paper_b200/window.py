@@ -12,7 +12,7 @@ between their KVM layers (the reference's own such mixers, model/swa_mixer.py, c
 
 All of it is bf16, on CUDA devices, inference only.  Calls only enqueue kernels on the current stream of the tensors' device;
 nothing is read back.  Positions and lengths are device tensors (int32, [batch]), so that a captured graph can be replayed
-with other ones, or one Python int for all sequences.
+with other ones; the cache's calls also take one Python int for all sequences.
 """
 
 from __future__ import annotations
@@ -117,8 +117,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
 
     q [B,Hq,T,D], k, v [B,Hkv,S,D] with S >= T; query t stands at position S - T + t.  (The earlier tokens of a chunk may be
     what ``WindowCache.read`` returns: positions only count relative to each other, as long as the sinks and the last
-    ``window - 1`` tokens are there.)  ``window`` None: every earlier token is visible.  ``lengths`` (int32 [B]): tokens of each
-    sequence, S at most; what lies behind them is padding, is never looked at, and its output rows are zeros.
+    ``window - 1`` tokens are there.  One call takes sequences that hold equally many of them, as all do that have passed
+    ``sinks + window`` tokens; others go one by one, without the zeros that ``read`` leaves behind a shorter one.)  ``window``
+    None: every earlier token is visible.  ``lengths`` (int32 [B]): tokens of each sequence, S at most; what lies behind them is
+    padding, is never looked at, and its output rows are zeros.
     Returns [B,T,Hq*D] (``out`` if given, which must not share memory with q, k or v)."""
     B, Hq, T, D = _shape4(q, "q", "[B,Hq,T,D]")
     _, Hkv, S, _ = _shape4(k, "k", "[B,Hkv,S,D]")
@@ -142,8 +144,10 @@ class WindowCache:
     """Keys and values of the first ``sinks`` and the last ``window`` tokens of ``batch`` sequences, in 16 bits or in 4 bits
     (4.5 with the scales; the format: include/kvm_b200.h).
 
-    The sequences' lengths are the caller's: every call is given positions or lengths, and none of them changes any.  Calls on
-    one cache run in the order of their streams; a call that writes must not overlap with another call on the same cache."""
+    The sequences' lengths are the caller's: every call is given positions or lengths, and none of them changes any.  A token
+    that is written takes the place of the one R before it for good, R being ``window`` rounded up to 16: a sequence that goes
+    back by more than R - window tokens misses what they pushed out.  Calls on one cache run in the order of their streams; a
+    call that writes must not overlap with another call on the same cache."""
 
     def __init__(self, batch: int, n_kv_heads: int, head_dim: int, *, window: int, sinks: int = 0, bits: int = 16, device="cuda"):
         self.batch, self.n_kv_heads, self.head_dim = _int32(batch, "batch"), _int32(n_kv_heads, "n_kv_heads"), _int32(head_dim, "head_dim")
@@ -186,8 +190,8 @@ class WindowCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, positions, lengths=None) -> None:
         """Writes tokens ``positions[b] ...`` of every sequence: k, v [B,Hkv,T,D], of which sequence b brings the first
-        ``lengths[b]`` (None: all).  A negative position leaves its sequence as it is.  Positions stay below 2^31 - T.  Tokens that
-        later ones of the call push out are not written."""
+        ``lengths[b]`` (None: all), from memory that is not the cache's own.  A negative position leaves its sequence as it is.
+        Positions stay below 2^31 - T.  Tokens that later ones of the call push out are not written."""
         T = _shape4(k, "k", "[B,Hkv,T,D]")[2]
         shape = (self.batch, self.n_kv_heads, T, self.head_dim)
         ka, va = _rows(k, "k", shape, self.device), _rows(v, "v", shape, self.device)
@@ -237,7 +241,8 @@ class WindowCache:
 
 
 def check_status(device="cuda") -> None:
-    """Synchronise and raise if a window kernel on the device reported a device-side timeout since the last check."""
+    """Synchronise and raise if a window kernel on the device, whoever called it, reported a device-side timeout since the last
+    check (one word per device, cleared by the check that reports it)."""
     dev = torch.device(device)
     dev = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
     _call(dev, _lib.load().kvm_window_status)
