@@ -370,7 +370,7 @@ struct Again {
   const PromptArgs& a;
   int b, hq, hkv, t, p, lo, ns, n;  // the keys that any of the rows sees: the first ns, then those from lo on
   float m, inv;
-  bool have;
+  bool have, large_q;  // (large_q: of any row's query)
   static constexpr unsigned kAll = 0xffffffffu;
   static constexpr int kKeys = 8;   // at a time: as many loads in flight
   __device__ __forceinline__ int key(int i) const { return i < ns ? i : lo + i - ns; }
@@ -399,6 +399,16 @@ struct Again {
 #pragma unroll
     for (int e = 0; e < kKeys; ++e) x[e] = __fmul_rn(s[e].x + s[e].y, a.scale_log2);
   }
+  // Is there a channel of 2^40 or more, an infinity or NaN?  (Of queries and keys below it no score passes fp32's range.)
+  static __device__ __forceinline__ bool beyond(const bf16* row, int D) {
+    unsigned top = 0;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 8) {
+      const uint4 y = *reinterpret_cast<const uint4*>(row + d);
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu), __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu)));
+    }
+    return max(top & 0xffffu, top >> 16) >= (127u + 40u) << 7;
+  }
   // is the score of key j -inf?
   __device__ __forceinline__ bool weightless(int j) const {
     const bf16 *qr = a.q.row(b, hq, t), *kr = a.k.row(b, hkv, j);
@@ -418,6 +428,7 @@ struct Again {
 #pragma unroll 2
     for (int i0 = 0; i0 < n; i0 += 32) {
       unsigned is_nan = 0, is_pos = 0, is_neg = 0;  // of the lane's key
+      bool may_be = false;                          // weightless, for some row
       if (i0 + lane < n) {
         const uint4* vr = reinterpret_cast<const uint4*>(a.v.row(b, hkv, key(i0 + lane)) + c0);
         uint4 y[4];
@@ -439,8 +450,10 @@ struct Again {
               else if (u == 0xff80u) is_neg |= bit;
             }
           }
+          may_be = large_q || beyond(a.k.row(b, hkv, key(i0 + lane)), a.D);
         }
       }
+      const unsigned doubt = __ballot_sync(kAll, may_be);
       unsigned hits = __ballot_sync(kAll, (is_nan | is_pos | is_neg) != 0);
       if (hits == 0) continue;
       for (; hits; hits &= hits - 1) {
@@ -449,7 +462,7 @@ struct Again {
         if (!sees(i0 + src)) continue;
         nan |= x;
         if ((y | z) == 0) continue;
-        if (weightless(key(i0 + src))) nan |= y | z;  // (0 x inf, of a key that is seen)
+        if ((doubt >> src & 1) && weightless(key(i0 + src))) nan |= y | z;  // (0 x inf, of a key that is seen)
         else { pos |= y; neg |= z; }
       }
       if (!__any_sync(kAll, bad & ~(nan | (pos & neg)))) break;  // (settled whatever follows)
@@ -545,7 +558,8 @@ __device__ __noinline__ void revisit(const PromptArgs& a, const int* pre, int n_
     if (!__any_sync(kAll, again)) continue;
     const int p_lo = __reduce_min_sync(kAll, again ? p : 0x7fffffff), p_hi = __reduce_max_sync(kAll, again ? p : -1);
     const int lo = max(0, p_lo - a.window + 1), ns = min(a.sinks, lo);
-    Again rows{a, it.b, hq, it.hkv, again ? t : 0, again ? p : -1, lo, ns, ns + p_hi + 1 - lo, 0.f, 0.f, false};
+    Again rows{a, it.b, hq, it.hkv, again ? t : 0, again ? p : -1, lo, ns, ns + p_hi + 1 - lo, 0.f, 0.f, false, false};
+    rows.large_q = __any_sync(kAll, again && Again::beyond(a.q.row(rows.b, rows.hq, rows.t), a.D));
 #pragma unroll 1
     for (int c0 = 0; c0 < a.D; c0 += 32) {
       const unsigned mine = !again ? 0 : c0 < 64 ? (c0 < 32 ? bad[0] : bad[1]) : (c0 < 96 ? bad[2] : bad[3]);
