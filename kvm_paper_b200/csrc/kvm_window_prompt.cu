@@ -352,13 +352,13 @@ __device__ __forceinline__ bool issue(const PromptArgs& a, const int* pre, int n
 }
 
 // ------------------------------------------------------------------------------------------ softmax
-// Rows to be formed again.  The tiles leave a mark in the first column that is concerned, a NaN that no conversion makes: the row's
-// scores are numbers, but not all of the tensor core's sums are.  An infinity or NaN among the values did that, of a key that the row sees or of one
-// that it does not (0 x inf), or sums beyond fp32.
-// Another mark in the first column asks for all of the row's columns: its maximum is beyond 2^16.  The tiles form a weight from a fused
-// product and difference, which lies off the rounded maximum by up to half a step: 2^-8 there, from 2^31 on more than a
-// weight holds.  The second pass rounds every score as it rounds the maximum.  (As a variant of the tiles' weights it took 1 to 5 % of
-// every prompt's time.)
+// Rows to be formed again.  The tiles leave a mark in the first column that is concerned, a NaN that no conversion makes: the
+// row's scores are numbers, but not all of the tensor core's sums are.  An infinity or NaN among the values did that, of a key that
+// the row sees or of one that it does not (0 x inf), or sums beyond fp32.
+// Another mark, in the first column, asks for all of the row's columns: its maximum is beyond 2^16.  The tiles form a weight from
+// a fused product and difference, which lies off the rounded maximum by up to half a step: 2^-8 there, from 2^31 on more than
+// a weight holds.  The second pass rounds every score as it rounds the maximum.  (As a variant of the tiles' weights it took 1 to
+// 5 % of every prompt's time.)
 constexpr unsigned kAgain = 0x7fc5, kAllAgain = 0x7fc6;
 constexpr float kFar = 0x1p16f;
 

@@ -621,9 +621,9 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[u][hb][e] = __fmul_rn(sc[u][hb][e], qs[hb][e & 1]);
           }
-        // ---- weights up to 2^kTop: the reference m is that much below the running maximum.  4 bits: f16 holds 2^-24 .. 2^15.
-        // 16 bits: small enough that 2^24 of the largest bf16 numbers stay inside fp32's range.  Of scores beyond 2^20 m is the
-        // maximum itself, which kTop could round away from by more than it says.
+        // ---- weights up to 2^kTop of the largest.  4 bits: f16 holds 2^-24 .. 2^15; the reference m is that much below the running
+        // maximum, but from 2^26 on, where the difference might be rounded beyond f16's range, the maximum itself.  16 bits:
+        // small enough that 2^24 of the largest bf16 numbers stay inside fp32's range; m is the maximum, kTop a sum of its own.
         constexpr float kTop = BITS == 4 ? 8.f : -24.f;
         float alpha[NH][2];
 #pragma unroll
@@ -643,7 +643,7 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
             x = fmaxf(x, __shfl_xor_sync(kAll, x, 16));
-            const float top = fmaxf(m[hb][e], fabsf(x) < 0x1p20f ? x - kTop : x);
+            const float top = fmaxf(m[hb][e], BITS == 4 && fabsf(x) < 0x1p26f ? x - kTop : x);
             alpha[hb][e] = ex2(m[hb][e] - top);
             m[hb][e] = top;
           }
@@ -668,7 +668,8 @@ kvm_window_token_kernel(WindowDev W, int G, Tensor4 q, Tensor4 k_new, Tensor4 v_
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-              const float2 x = __fadd2_rn(make_float2(sc[u][hb][e], sc[u][hb][e + 1]), make_float2(-m[hb][0], -m[hb][1]));
+              float2 x = __fadd2_rn(make_float2(sc[u][hb][e], sc[u][hb][e + 1]), make_float2(-m[hb][0], -m[hb][1]));
+              if (BITS == 16) x = __fadd2_rn(x, make_float2(kTop, kTop));
               p[e] = ex2(x.x);
               p[e + 1] = ex2(x.y);
             }

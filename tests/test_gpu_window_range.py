@@ -332,3 +332,21 @@ def test_prompt_of_nothing_but_infinities_costs_little():
     v = torch.full((1, 2, T, 128), math.inf, device="cuda", dtype=torch.bfloat16)
     got, ms = _timed(lambda: window.window_attention(q, k, v, window=None))
     assert bool((got == math.inf).all()) and ms < 16.0
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 20, 2.0 ** 24, 2.0 ** 26, 2.0 ** 27, 2.0 ** 28])
+def test_token_equal_large_scores_of_values_near_the_largest_number(bits, size):
+    """Keys that share the weight, however large their scores: sums that are not normalised yet stay in range."""
+    from kvm_paper_b200 import window
+    n, dim = 700, 64
+    k, v = torch.zeros(1, 1, n, dim, device="cuda", dtype=torch.bfloat16), torch.full((1, 1, n, dim), 3e38, device="cuda", dtype=torch.bfloat16)
+    v[..., 32:] = -3e38
+    k[..., 5] = 6.0  # (a scale of 1 and the largest level: exact)
+    q = torch.zeros(1, 3, 1, dim, device="cuda", dtype=torch.bfloat16)
+    q[..., 5] = torch.tensor([size, size * 1.5, -size], device="cuda").view(1, 3, 1)
+    c = window.WindowCache(1, 1, dim, window=n, bits=bits)
+    c.write(k, v, 0)
+    got = c.attend(q, n, scale=0.25).view(3, dim)
+    held = c.read(n)[1][0, 0, :1]
+    assert torch.allclose(got.double(), held.double().expand(3, dim), rtol=2 * wh.U_BF16, atol=0)
