@@ -528,8 +528,8 @@ struct Again {
 };
 
 // The marked rows of a softmax warp, once its tiles are done: nobody waits for it any more, however long it takes.  For 32 rows of
-// 128 channels: 12 ns per key and 32 columns to look through the values, 2.1 us per key to sum 32 columns again, 1.1 us for each
-// further 32 (of 8192 keys 17.7 ms, all columns 45 ms).  Inside the tiles' loop a call took 2 to 4 % of every prompt's time.
+// 128 channels: 14 ns per key and 32 columns to look through the values, 2.1 us per key to sum 32 columns again, 1.1 us for each
+// further 32 (of 8192 keys 18 ms, all columns 46 ms).  Inside the tiles' loop a call took 2 to 4 % of every prompt's time.
 template <bool LISTED>
 __device__ __noinline__ void revisit(const PromptArgs& a, const int* pre, int n_items, int I, int row, int lane) {
   constexpr unsigned kAll = 0xffffffffu;

@@ -16,7 +16,7 @@
 // weights down to 2^-22 of the largest keep all their bits, smaller ones an error of 2^-31 R and 2^-33 of the largest.
 // The new token: the CTA that reads the chunk with its row patches the stage and writes the row to memory.
 //
-// Measured: 4 bits, 64 x 4 kv rows of 16384 x 128 130 us (4.6 TB/s of codes and scales), one sequence of 262144 x 8 kv rows 69 us
+// Measured: 4 bits, 64 x 4 kv rows of 16384 x 128 132 us (4.6 TB/s of codes and scales), one sequence of 262144 x 8 kv rows 69 us
 // (4.4 TB/s): half of the ALU's and of the issue slots go into unpacking codes, the rest is the latency of a warp's dependent
 // steps, for which the registers leave room for eight warps.  16 bits, 64 x 4 kv rows of 4100 x 128 80 us (6.7 TB/s): memory.  A
 // few hundred tokens: 5 to 7 us, launch and two round trips to memory.
